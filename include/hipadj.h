@@ -447,6 +447,65 @@ int hipadj_comm_selfcheck(hipadj_handle *h);
  * once call k + 2 has been enqueued and the handle's stream has reached it.  on = 0 (default): in-stream, dp complete in stream order.  ABI 107. */
 int hipadj_comm_overlap(hipadj_handle *h, int on);
 
+/* Operators of sequence models next to the solves.  They have no handle: device pointers, sizes and strides in ELEMENTS, the caller's stream (NULL: the null stream) and the caller's
+ * workspace, which a call may overwrite and which belongs to it until its work on the stream is done; asynchronous, capturable, nothing is kept between calls.  `device` is made
+ * current inside the call and the caller's device again afterwards.  Errors: hipadj_last_error(NULL). */
+typedef enum { HIPADJ_F64 = 0, HIPADJ_F32 = 1, HIPADJ_BF16 = 2, HIPADJ_F16 = 3 } hipadj_dtype;
+typedef enum { HIPADJ_GATE_DECAY = 0, HIPADJ_GATE_LOG = 1, HIPADJ_GATE_SIGMOID = 2 } hipadj_gate; /* a = g, exp(g), 1 / (1 + exp(-g)) */
+
+/* The gated linear recurrence  h_t = a_t h_{t-1} + b_t  of every channel, b_t = x_t or, coupled, (1 - a_t) x_t: the diagonal linear system h' = r (x - h) stepped exactly (gate
+ * = -r dt, HIPADJ_GATE_LOG, coupled) — the forward solve, its adjoint (discretize-then-optimize: exact gradients of the states) and a single step of it.
+ *   dense   batch rows of `length` steps: x, gate, h, dh, dx, dgate [batch][length][channels] with the strides below (the channel stride is 1; an INPUT stride may be 0); h0, h_final,
+ *           dh_final, dh0 [batch][channels]
+ *   packed  nseq > 0, batch = 1: sequence s is the rows offsets[s] <= t < offsets[s + 1] (device memory, ascending; equal neighbours: an empty sequence, whose final state is its
+ *           first); h0, h_final, dh_final, dh0 [nseq][channels].  Rows of no sequence have h = 0 and zero gradients and are not used.  Offsets that do not ascend or pass `length` give
+ *           unspecified results, never an access outside the arrays.
+ * dtype: x, h, dh, dx; gate_dtype: gate, dgate — the same, or F32 next to BF16 / F16.  h0, h_final, dh_final, dh0 and the checkpoints: F64 for F64, else F32, contiguous.  States and
+ * gradients are carried in that type, the outputs rounded once.
+ *   hipadj_recurrence_sizes         bytes of the checkpoints and of the workspace (8-byte aligned; 0: none) of a configuration
+ *   hipadj_recurrence_forward_dev   h and h_final; h0 NULL = zeros; checkpoints NULL when no adjoint follows
+ *   hipadj_recurrence_adjoint_dev   the gradients dx, dgate, dh0 (each may be NULL) of sum(dh h) + sum(dh_final h_final); dh / dh_final NULL = zeros; h itself is not needed: each
+ *                                   checkpoint interval is re-solved
+ *   hipadj_recurrence_step_dev      one step of `batch` sequences: state[slots[i]] <- a state[slots[i]] + b, h[i] = the new state; x, gate, h [batch][channels], state [nslots][channels]
+ *                                   (F64 for F64, else F32) with row strides; slots NULL: row i has state i.  A slot outside [0, nslots) is padding: h[i] = 0.  Rows with the same
+ *                                   slot are consecutive steps of it in row order.  h may not overlap another argument. */
+typedef struct {
+    uint32_t struct_size;      /* = sizeof(hipadj_recurrence) */
+    int32_t device;
+    int32_t dtype, gate_dtype; /* hipadj_dtype */
+    int32_t gate;              /* hipadj_gate */
+    int32_t coupled;
+    int64_t batch, length, channels;
+    int64_t nseq;              /* packed sequences, 0: dense */
+    const void *offsets;       /* device [nseq + 1] */
+    int32_t offsets_bits;      /* 32 or 64 */
+    int32_t reserved;
+    int64_t x_stride[2], gate_stride[2], h_stride[2], dh_stride[2], dx_stride[2], dgate_stride[2]; /* batch, time */
+} hipadj_recurrence;
+int hipadj_recurrence_sizes(const hipadj_recurrence *r, int64_t *checkpoint_bytes, int64_t *workspace_bytes);
+int hipadj_recurrence_forward_dev(const hipadj_recurrence *r, const void *x, const void *gate, const void *h0, void *h, void *h_final, void *checkpoints, void *workspace, void *stream);
+int hipadj_recurrence_adjoint_dev(const hipadj_recurrence *r, const void *x, const void *gate, const void *h0, const void *checkpoints, const void *dh, const void *dh_final,
+                                  void *dx, void *dgate, void *dh0, void *workspace, void *stream);
+int hipadj_recurrence_step_dev(int32_t device, int32_t dtype, int32_t gate_dtype, int32_t gate_form, int32_t coupled, int64_t batch, int64_t channels, const void *x, int64_t x_stride,
+                               const void *gate, int64_t gate_stride, void *state, int64_t state_stride, int64_t nslots, const void *slots, int32_t slots_bits, void *h, int64_t h_stride,
+                               void *stream);
+
+/* The orthogonalised update of weight matrices (the step after a gradient dp of a model's weights): with the momentum m <- beta m + g and u = g + beta m (nesterov) or m,
+ *   X = u / (|u|_F + 1e-7),  `steps` times  X <- c0 X + c1 A X + c2 A A X  with A = X X' (X' X when that is smaller),  out = scale X
+ * — the nearest semi-orthogonal matrix up to the factors the coefficients leave (for (3.4445, -4.7750, 2.0315): singular values in 0.7 ... 1.2).  grad, out [batch][rows][cols] of dtype
+ * F32, BF16 or F16, momentum the same shape in F32 (NULL: none), column stride 1, rows and matrices strided.  Arithmetic: products of two-term F16 splits (22 bits) accumulated
+ * in F32; for BF16 with both sides of at least 256, one F16 term a factor, whose rounding adds about as much as the output's own.  A matrix with a non-finite entry gives NaN. */
+typedef struct {
+    uint32_t struct_size;      /* = sizeof(hipadj_orthogonal) */
+    int32_t device, dtype, steps, nesterov, reserved;
+    int64_t batch, rows, cols;
+    int64_t grad_stride[2], momentum_stride[2], out_stride[2]; /* matrix, row */
+    double beta, scale;
+    const double *coefficients; /* host [steps][3] */
+} hipadj_orthogonal;
+int hipadj_orthogonalized_update_size(const hipadj_orthogonal *o, int64_t *workspace_bytes);
+int hipadj_orthogonalized_update_dev(const hipadj_orthogonal *o, const void *grad, float *momentum, void *out, void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

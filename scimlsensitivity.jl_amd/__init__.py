@@ -12,6 +12,7 @@ from .problems import (RK4, ETDRK4, Tsit5, Rosenbrock23, DeviceFunction, WideDev
 from .engine import Engine
 from .interface import solve, adjoint_sensitivities, concrete_solve_adjoint, make_autograd_function
 from .events import EventSolution
+from .operators import RecurrenceSolution, recurrence_solve, recurrence_adjoint, gated_recurrence, gated_recurrence_step, orthogonalized_update, NEWTON_SCHULZ
 from .distributed import shard_range, allreduce_dp, gather_du0, comm_unique_id, init_native_allreduce
 from . import build as _build
 
@@ -23,4 +24,5 @@ __all__ = [
     "QuadratureAdjoint", "GaussAdjoint", "GaussKronrodAdjoint", "ischeckpointing", "RK4", "ETDRK4", "Tsit5", "Rosenbrock23", "DeviceFunction", "WideDeviceFunction", "ODEProblem", "EnsembleProblem",
     "EnsembleSolution", "ContinuousCallback", "LsqShift", "LsqData", "ModelLoss", "HalfSquaredSum", "FirstStateSquaredPlusFirstParam", "ModelCost", "Engine", "solve", "adjoint_sensitivities", "concrete_solve_adjoint",
     "make_autograd_function", "shard_range", "allreduce_dp", "gather_du0", "comm_unique_id", "init_native_allreduce", "build_extension",
+    "RecurrenceSolution", "recurrence_solve", "recurrence_adjoint", "gated_recurrence", "gated_recurrence_step", "orthogonalized_update", "NEWTON_SCHULZ",
 ]

@@ -25,6 +25,8 @@ DECLARED_SYMBOLS = (
     "hipadj_model_set_discrete_loss", "hipadj_model_set_discrete_loss_function", "hipadj_wmodel_set_discrete_loss", "hipadj_set_loss_data", "hipadj_set_loss_data_dev",
     "hipadj_loss_value", "hipadj_loss_value_dev", "hipadj_adjoint_dev_soa", "hipadj_soa_stride", "hipadj_device_count", "hipadj_wmodel_declare_dense_chain",
     "hipadj_model_set_continuous_callback", "hipadj_model_set_vector_continuous_callback", "hipadj_model_set_callback_direction", "hipadj_event_counts", "hipadj_event_states", "hipadj_event_components", "hipadj_set_event_cotangents",
+    "hipadj_recurrence_sizes", "hipadj_recurrence_forward_dev", "hipadj_recurrence_adjoint_dev", "hipadj_recurrence_step_dev",
+    "hipadj_orthogonalized_update_size", "hipadj_orthogonalized_update_dev",
 )
 
 
@@ -56,6 +58,25 @@ class HipadjStats(C.Structure):
         ("adjoint_main_kernel_ms_last", C.c_double), ("adjoint_main_kernel_ms_total", C.c_double),
         ("adjoint_algorithmic_bytes", C.c_double), ("vjp_steps", C.c_double), ("workspace_bytes", C.c_double),
         ("launches_per_pass", C.c_int32), ("routed_family", C.c_int32),
+    ]
+
+
+class HipadjRecurrence(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("gate_dtype", C.c_int32), ("gate", C.c_int32), ("coupled", C.c_int32),
+        ("batch", C.c_int64), ("length", C.c_int64), ("channels", C.c_int64), ("nseq", C.c_int64),
+        ("offsets", C.c_void_p), ("offsets_bits", C.c_int32), ("reserved", C.c_int32),
+        ("x_stride", C.c_int64 * 2), ("gate_stride", C.c_int64 * 2), ("h_stride", C.c_int64 * 2),
+        ("dh_stride", C.c_int64 * 2), ("dx_stride", C.c_int64 * 2), ("dgate_stride", C.c_int64 * 2),
+    ]
+
+
+class HipadjOrthogonal(C.Structure):
+    _fields_ = [
+        ("struct_size", C.c_uint32), ("device", C.c_int32), ("dtype", C.c_int32), ("steps", C.c_int32), ("nesterov", C.c_int32), ("reserved", C.c_int32),
+        ("batch", C.c_int64), ("rows", C.c_int64), ("cols", C.c_int64),
+        ("grad_stride", C.c_int64 * 2), ("momentum_stride", C.c_int64 * 2), ("out_stride", C.c_int64 * 2),
+        ("beta", C.c_double), ("scale", C.c_double), ("coefficients", C.POINTER(C.c_double)),
     ]
 
 
@@ -143,6 +164,13 @@ def load():
     L.hipadj_adjoint_dev_soa.argtypes = [vp, vp, vp, vp]
     L.hipadj_soa_stride.argtypes = [vp, C.POINTER(C.c_int64)]
     L.hipadj_device_count.restype = C.c_int
+    i64, i32 = C.c_int64, C.c_int32
+    L.hipadj_recurrence_sizes.argtypes = [C.POINTER(HipadjRecurrence), C.POINTER(i64), C.POINTER(i64)]
+    L.hipadj_recurrence_forward_dev.argtypes = [C.POINTER(HipadjRecurrence)] + [vp] * 8
+    L.hipadj_recurrence_adjoint_dev.argtypes = [C.POINTER(HipadjRecurrence)] + [vp] * 11
+    L.hipadj_recurrence_step_dev.argtypes = [i32, i32, i32, i32, i32, i64, i64, vp, i64, vp, i64, vp, i64, i64, vp, i32, vp, i64, vp]
+    L.hipadj_orthogonalized_update_size.argtypes = [C.POINTER(HipadjOrthogonal), C.POINTER(i64)]
+    L.hipadj_orthogonalized_update_dev.argtypes = [C.POINTER(HipadjOrthogonal)] + [vp] * 5
     _lib = L
     return L
 

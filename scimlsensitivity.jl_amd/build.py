@@ -19,11 +19,13 @@ LIB = os.environ.get("HIPADJ_BUILD_LIB") or os.path.join(HERE, "libhipadj.so")
 OBJ = os.path.join(HERE, "build") if "HIPADJ_BUILD_LIB" not in os.environ else os.path.join(HERE, "build_ab", os.path.splitext(os.path.basename(LIB))[0])   # build_ab/: git- and gpurun-ignored
 
 DEPS = sorted(glob.glob(os.path.join(CSRC, "*.h*"))) + [os.path.join(CSRC, "hipadj.map")] + [os.path.join(os.path.dirname(HERE), "include", "hipadj.h"), os.path.abspath(__file__)]
-FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + os.environ.get("HIPADJ_BUILD_EXTRA", "").split()
+# -packed-fp32-ops: some forms of the packed 32-bit instructions have given wrong results on this hardware (the host pass warns that it does not know the feature)
+FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + os.environ.get("HIPADJ_BUILD_EXTRA", "").split()
 
 LANE_MODELS = ["ModelLV", "ModelLVT", "ModelLorenz", "ModelLinDiag", "ModelFallMass"]   # csrc/hipadj_models.hpp
 FIELD_GRIDS = [8, 16, 32]
 MLP_HIDDEN = [32, 64, 128]
+REC_PAIRS = ["F64", "F32", "BF16", "BF16_F32", "F16", "F16_F32"]   # (x, gate) types of the recurrence: rec::PAIR_* of csrc/hipadj_recurrence.hpp
 
 
 def units():
@@ -38,10 +40,23 @@ def units():
     for g in sorted(FIELD_GRIDS, reverse=True):
         u.append((f"field_{g}.o", "hipadj_tu_family.hip", [f"-DHIPADJ_TU_FIELD={g}"]))
     u.append(("api.o", "hipadj_api.hip", []))
+    for p in REC_PAIRS:
+        u.append((f"recurrence_{p}.o", "hipadj_tu_recurrence.hip", [f"-DHIPADJ_TU_PAIR=rec::PAIR_{p}"]))
+    u.append(("recurrence.o", "hipadj_tu_recurrence.hip", []))
+    u.append(("orthogonal.o", "hipadj_tu_orthogonal.hip", []))
     return u
 
 
 API_ONLY = {"hipadj_user.hpp", "hipadj_dual.hpp", "hipadj_comm.hpp", "hipadj_api.hip"}   # included by hipadj_api.hip alone
+
+
+OPS_ONLY = {"hipadj_tu_recurrence.hip": {"hipadj_recurrence.hpp", "hipadj_ops.hpp"}, "hipadj_tu_orthogonal.hip": {"hipadj_orthogonal.hpp", "hipadj_ops.hpp"}}   # all that these units include
+
+
+def _sees(src, header):
+    if src in OPS_ONLY:
+        return header in OPS_ONLY[src]
+    return header not in set().union(*OPS_ONLY.values())
 
 
 def _stale(obj, src):
@@ -55,6 +70,8 @@ def _stale(obj, src):
         if b.endswith(".hip") and d != src:
             continue
         if not api and b in API_ONLY:
+            continue
+        if b.endswith(".hpp") and not _sees(os.path.basename(src), b):
             continue
         if os.path.exists(d) and os.path.getmtime(d) > t:
             return True

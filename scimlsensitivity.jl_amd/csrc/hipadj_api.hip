@@ -17,6 +17,7 @@
 #include "hipadj_route.hpp"
 
 static thread_local std::string g_create_error;
+void ops_set_error(const char* text) { g_create_error = text; }   // operators without a handle (hipadj_ops.hpp)
 static int user_prepare(hipadj_handle* h);   // hiprtc compilation of the kernels of a runtime-registered model
 static bool fused_eligible(const hipadj_config* cfg, const Plan& P);   // which sweeps finish their reverse pass in one launch
 static int wide_prepare(hipadj_handle* h);   // ... of a wide model (workgroup-per-trajectory family, hipadj_wide.hpp)

@@ -1,0 +1,591 @@
+// hipadj_recurrence.hpp — the gated linear recurrence: the exactly stepped diagonal linear system of a sequence model, its adjoint and its single step.
+//
+//   h_t = a_t h_{t-1} + b_t,   a = g | exp(g) | sigmoid(g),   b = x | (1 - a) x
+//
+// and, with the cotangents dh_t of all states and dh_T of the last one,
+//
+//   G_t = dh_t + R_{t+1},  R_t = a_t G_t  (R_{T+1} = dh_T),   dx_t = G_t (1 - a_t or 1),   da_t = G_t (h_{t-1} [- x_t]),   dh_0 = R_1.
+//
+// Both directions are scans of affine maps h -> A h + H, whose composition is associative, so the time axis can be cut:
+//   * a workgroup takes a TILE of NW * TS rows (TS: TSF or TSA) by 64 * V channels; wave w holds rows [w TS, (w + 1) TS) of it in registers, every lane V neighbouring channels, so that each
+//     row of a wave is one contiguous request and every input is read from memory ONCE;
+//   * the NW partial maps of a tile are joined through LDS;
+//   * the tiles of one (batch row, channel group) form a CHAIN.  A tile first publishes its own map (A, H); the state at its start is the state at the start of its group of
+//     GS tiles carried through the maps of the group's earlier tiles, in this fixed order — the result does not depend on which tile ran first — and the last tile of a group
+//     publishes the state at the next group's start.  A long axis therefore costs one exchange per GROUP on the critical path, not one per tile.
+// Tiles are handed out by a ticket (one atomic increment per workgroup) in an order where a tile only ever waits for tiles with lower tickets: those already run, and the
+// publication of a map waits for nothing, so every wait ends.  A published value travels in 64-bit words of 32 bits of data and a non-zero tag, written and read as relaxed
+// device-scope atomics: a word is complete or absent, nothing orders one word against another and no cache has to be written back.  The words are zeroed by a launch of their own.
+//
+// The adjoint does not read h: the forward pass leaves the state at the start of every TTA rows (the checkpoints, 1 / TTA of h in 32 bits) and a tile of the adjoint re-solves its rows from there in
+// registers — the bytes of reading h back are those of reading x, and the states are the unrounded ones.
+// Bound: memory, 3 streams forward and 5 in the adjoint.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace rec {
+
+constexpr int NW = 8;             // waves of a workgroup = time pieces of a tile
+constexpr int TSF = 16;           // rows of a piece, forward: (a, b) of 16 x V cells fit the 128 registers that leave room for two workgroups a CU
+constexpr int TSA = 8;            // rows of a piece, adjoint: five values a cell, so half as many (16 spilled 47 ... 101 registers and left one workgroup a CU)
+constexpr int TTF = NW * TSF, TTA = NW * TSA;                 // rows of a tile; a checkpoint every TTA rows
+constexpr int NT = NW * 64;
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+struct Args {
+    const void *x, *gate, *h0, *dh, *dh_final;
+    void *h, *h_final, *dx, *dgate, *dh0, *ckpt;
+    const void* offsets;                                     // [nseq + 1], offsets64: 64-bit
+    int64_t x_sb, x_st, g_sb, g_st, h_sb, h_st, dh_sb, dh_st, dx_sb, dx_st, dg_sb, dg_st;
+    int64_t L, D, nseq;
+    int32_t offsets64, ntiles, nckpt, ncg, nchains, GS;      // nckpt: checkpoints of a batch row; ncg: channel groups; nchains = batch * ncg; GS: tiles of a group
+    uint64_t *agg, *car;                                     // [nchains][ntiles][2 * WPV][CW], [nchains][ngroups][WPV][CW]
+    uint32_t* ticket;
+};
+
+template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+// ---- values -----------------------------------------------------------------------------------------------------------------------------------------------------
+
+// exp in 32 bits: exp2 of g log2(e) with the product's rounding error carried along, so that strong decays keep their digits; beyond +-200 (0 or inf in 32 bits) the argument is
+// cut off, which also keeps the error term finite for a gate of -inf or of its type's lowest value.  NaN stays NaN.
+__device__ inline float exp_(float g) {
+    g = g < -200.f ? -200.f : (g > 200.f ? 200.f : g);
+    const float p = g * 1.44269504f;
+    const float e = fmaf(g, 1.44269504f, -p) + g * 1.92596299e-8f;
+    const float r = __builtin_amdgcn_exp2f(p);
+    return fmaf(r, e * 0.693147181f, r);
+}
+__device__ inline double exp_(double g) { return exp(g); }
+// 1 - exp(g) without the cancellation at small |g| (Taylor series; the first term left out is below 2e-8 of the value at 0.35)
+__device__ inline float one_minus_exp(float g, float a) {
+    float s = fmaf(g, 1.f / 5040.f, 1.f / 720.f);
+    s = fmaf(s, g, 1.f / 120.f); s = fmaf(s, g, 1.f / 24.f); s = fmaf(s, g, 1.f / 6.f); s = fmaf(s, g, 0.5f); s = fmaf(s, g, 1.f);
+    return fabsf(g) < 0.35f ? -g * s : 1.f - a;
+}
+__device__ inline double one_minus_exp(double g, double) { return -expm1(g); }
+__device__ inline float recip(float x) { return __builtin_amdgcn_rcpf(x); }
+__device__ inline double recip(double x) { return 1.0 / x; }
+__device__ inline float neg_abs(float x) { return -fabsf(x); }
+__device__ inline double neg_abs(double x) { return -fabs(x); }
+
+// a and 1 - a of a gate; `rest` is only formed where it is used.  A decay next to one acts over hundreds of rows, so its last bit counts: where 1 - a is the smaller one it is formed
+// first, with its own relative accuracy, and a as its difference from one, within half a unit of the last place.
+template <int FORM, bool REST, class S> __device__ inline void decay(S g, S& a, S& rest) {
+    if constexpr (FORM == 0) { a = g; if constexpr (REST) rest = S(1) - g; }
+    else if constexpr (FORM == 1) {
+        a = exp_(g);
+        if constexpr (REST) { rest = one_minus_exp(g, a); a = fabs(g) < S(0.35) ? S(1) - rest : a; }
+    } else { const S e = exp_(neg_abs(g)), s = e * recip(S(1) + e), l = S(1) - s; a = g >= S(0) ? l : s; if constexpr (REST) rest = g >= S(0) ? s : l; }
+}
+
+// ---- published words ----------------------------------------------------------------------------------------------------------------------------------------------
+
+template <class S> constexpr int WPV = sizeof(S) / 4;         // words of a value
+__device__ inline void put(uint64_t* w, uint64_t v) { __hip_atomic_store(w, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ inline uint64_t get(const uint64_t* w) { return __hip_atomic_load(const_cast<uint64_t*>(w), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ inline void publish(uint64_t* w, int64_t cw, float v, uint32_t tag) { put(w, (uint64_t(tag) << 32) | __float_as_uint(v)); }
+__device__ inline void publish(uint64_t* w, int64_t cw, double v, uint32_t tag) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    put(w, (uint64_t(tag) << 32) | (b & 0xffffffffu)); put(w + cw, (uint64_t(tag) << 32) | (b >> 32));
+}
+// waits for a published value; every wave that waits does so for a tile with a lower ticket (top of this file)
+__device__ inline uint32_t await_value(const uint64_t* w, int64_t, float& v) {
+    uint64_t q;
+    while (!((q = get(w)) >> 32)) __builtin_amdgcn_s_sleep(1);
+    v = __uint_as_float((uint32_t)q);
+    return (uint32_t)(q >> 32);
+}
+__device__ inline uint32_t await_value(const uint64_t* w, int64_t cw, double& v) {
+    uint64_t q, r;
+    while (!((q = get(w)) >> 32)) __builtin_amdgcn_s_sleep(1);
+    while (!((r = get(w + cw)) >> 32)) __builtin_amdgcn_s_sleep(1);
+    v = __longlong_as_double((long long)((q & 0xffffffffu) | (r << 32)));
+    return (uint32_t)(q >> 32);
+}
+constexpr uint32_t TAG_MAP = 1, TAG_CUT = 2;                  // CUT: no state passes (a sequence starts inside): H alone, whatever A and the state are
+
+// ---- packed sequences ---------------------------------------------------------------------------------------------------------------------------------------------
+
+__device__ inline int64_t offset_at(const Args& p, int64_t i) { return p.offsets64 ? ((const int64_t*)p.offsets)[i] : (int64_t)((const int32_t*)p.offsets)[i]; }
+
+// the first sequence that ends behind row t (nseq: none), found by a 64-ary search over the ends; offsets that do not ascend give some number in [0, nseq]
+__device__ inline int64_t seq_behind(const Args& p, int64_t t) {
+    int64_t lo = 0, n = p.nseq;                               // the answer is in [lo, lo + n]
+    const int lane = threadIdx.x & 63;
+    while (n > 0) {
+        const int64_t step = (n + 63) / 64;
+        const int64_t i = lo + (int64_t)lane * step + step - 1;                     // last of this lane's stretch
+        const bool in = (int64_t)lane * step < n;
+        const int64_t last = i < lo + n ? i : lo + n - 1;
+        const bool before = in && offset_at(p, last + 1) <= t;                      // the whole stretch ends at t or earlier
+        const int k = __popcll(__ballot(before));
+        const int64_t at = (int64_t)k * step;
+        if (at >= n) return lo + n;
+        lo += at;
+        n = (step < n - at ? step : n - at) - 1;                                    // its last one ends behind t
+    }
+    return lo;
+}
+
+struct Marks { uint32_t start, end, out; };                   // bits of a piece's rows: first of a sequence, last of one, of none
+template <int TS> __device__ inline Marks marks_of(const Args& p, int64_t t0) {
+    Marks m{0, 0, (1u << TS) - 1};
+    int64_t pos = t0;
+    while (pos < t0 + TS && pos < p.L) {                      // pos advances in every turn, whatever the offsets hold
+        const int64_t s = seq_behind(p, pos);
+        if (s >= p.nseq) break;
+        const int64_t st = offset_at(p, s), en = offset_at(p, s + 1);
+        const int64_t from = st > pos ? st : pos, to = en < t0 + TS ? en : t0 + TS;
+        for (int64_t t = from; t < to; ++t) m.out &= ~(1u << (int)(t - t0));
+        if (st >= t0 && st < to) m.start |= 1u << (int)(st - t0);
+        if (en - 1 >= from && en - 1 < t0 + TS) m.end |= 1u << (int)(en - 1 - t0);
+        pos = en > pos ? en : pos + 1;
+    }
+    for (int i = 0; i < TS; ++i) if (t0 + i >= p.L) { m.out |= 1u << i; m.start &= ~(1u << i); m.end &= ~(1u << i); }
+    m.start = __builtin_amdgcn_readfirstlane(m.start); m.end = __builtin_amdgcn_readfirstlane(m.end); m.out = __builtin_amdgcn_readfirstlane(m.out);
+    return m;
+}
+
+// ---- the scan over the tiles of a chain -----------------------------------------------------------------------------------------------------------------------------
+
+template <class S, int V> struct Lds {
+    S A[NW][64 * V], H[NW][64 * V];                           // maps of the pieces
+    S pA[NW][64 * V], pH[NW][64 * V];                         // maps of the group's earlier tiles, NW at a time
+    S c[64 * V];                                              // state at the group's start
+    uint32_t cut[NW], pcut[NW];
+    uint32_t ticket;
+};
+
+template <class S> __device__ inline S through(S A, S H, uint32_t cut, S c) { return cut ? H : A * c + H; }
+
+// The state at the start of position `k` of chain `c` (positions are in scan order; the adjoint counts tiles from the end), given the maps of its NW pieces in sh.A / sh.H / sh.cut
+// (piece order is scan order too).  `first`: the state at the chain's start.  Publishes what later tiles of the chain wait for.  Returns with all pieces' waves past a barrier.
+template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>& sh, int64_t c, int k, const S (&first)[V], S (&carry)[V]) {
+    constexpr int CW = 64 * V, W = WPV<S>;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, ch = lane * V;
+    const int g = k / p.GS, base = g * p.GS, before = k - base, ngroups = (p.ntiles + p.GS - 1) / p.GS;
+    const bool last = k == p.ntiles - 1, closes = !last && before == p.GS - 1;
+    __syncthreads();
+    S A[V], H[V];
+    uint32_t cut = 0;
+    if (wave == 0 && !last) {                                 // the tile's own map
+#pragma unroll
+        for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+        for (int w = 0; w < NW; ++w) {
+            const uint32_t q = sh.cut[w];
+            cut |= q;
+#pragma unroll
+            for (int v = 0; v < V; ++v) { H[v] = through(sh.A[w][ch + v], sh.H[w][ch + v], q, H[v]); A[v] = q ? S(0) : A[v] * sh.A[w][ch + v]; }
+        }
+        if (!closes) {                                        // (only later tiles of the same group read it)
+            uint64_t* dst = p.agg + (c * p.ntiles + k) * (2 * W) * CW + ch;
+#pragma unroll
+            for (int v = 0; v < V; ++v) { publish(dst + v, CW, A[v], cut ? TAG_CUT : TAG_MAP); publish(dst + W * CW + v, CW, H[v], TAG_MAP); }
+        }
+    }
+    S st[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) st[v] = first[v];
+    for (int j0 = 0; j0 == 0 || j0 < before; j0 += NW) {
+        const int j = j0 + wave;
+        if (j < before) {
+            const uint64_t* src = p.agg + (c * p.ntiles + base + j) * (2 * W) * CW + ch;
+            uint32_t q = 0;
+#pragma unroll
+            for (int v = 0; v < V; ++v) { q = await_value(src + v, CW, sh.pA[wave][ch + v]); await_value(src + W * CW + v, CW, sh.pH[wave][ch + v]); }
+            if (lane == 0) sh.pcut[wave] = q == TAG_CUT;
+        }
+        if (j0 == 0 && g > 0 && wave == (before < NW ? before : NW - 1)) {
+            const uint64_t* src = p.car + (c * ngroups + g) * W * CW + ch;
+#pragma unroll
+            for (int v = 0; v < V; ++v) await_value(src + v, CW, sh.c[ch + v]);
+        }
+        __syncthreads();
+        if (j0 == 0 && g > 0) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) st[v] = sh.c[ch + v];
+        }
+        for (int i = 0; i < NW && j0 + i < before; ++i) {
+            const uint32_t q = sh.pcut[i];
+#pragma unroll
+            for (int v = 0; v < V; ++v) st[v] = through(sh.pA[i][ch + v], sh.pH[i][ch + v], q, st[v]);
+        }
+        if (j0 + NW < before) __syncthreads();                // the next NW maps take the same place
+    }
+    if (wave == 0 && closes) {
+        uint64_t* dst = p.car + (c * ngroups + g + 1) * W * CW + ch;
+#pragma unroll
+        for (int v = 0; v < V; ++v) publish(dst + v, CW, through(A[v], H[v], cut, st[v]), TAG_MAP);
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) carry[v] = st[v];
+}
+
+// the tile of this workgroup: chain and position in scan order
+template <class S, int V> __device__ inline void take(const Args& p, Lds<S, V>& sh, int64_t& c, int& k) {
+    if (p.ntiles == 1) { c = blockIdx.x; k = 0; return; }
+    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.ticket, 1u);
+    __syncthreads();
+    const uint32_t t = __builtin_amdgcn_readfirstlane(sh.ticket);
+    c = t % (uint32_t)p.nchains; k = (int)(t / (uint32_t)p.nchains);
+}
+
+template <class T, int V> __device__ inline Pack<T, V> read(const void* base, int64_t at) { return *(const Pack<T, V>*)((const T*)base + at); }
+
+// ---- forward ------------------------------------------------------------------------------------------------------------------------------------------------------
+
+template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
+__global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Args p) {
+    __shared__ Lds<S, V> sh;
+    constexpr int CW = 64 * V, TS = TSF;
+    int64_t c; int k;
+    take(p, sh, c, k);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t b = c / p.ncg, cg = c % p.ncg, ch = cg * CW + lane * V;
+    const bool on = ch < p.D;
+    const int64_t cl = on ? ch : 0;                           // lanes past the last channel read the first one and write nothing
+    const int64_t t0 = (int64_t)k * TTF + wave * TS;
+    const int64_t xo = b * p.x_sb + t0 * p.x_st + cl, go = b * p.g_sb + t0 * p.g_st + cl;
+    S a[TS][V], u[TS][V];                                     // (a, b) of each row
+    Marks m{0, 0, 0};
+    if constexpr (PACKED) m = marks_of<TS>(p, t0);
+    const bool whole = t0 + TS <= p.L;
+    Pack<T, V> rx[TS]; Pack<TG, V> rg[TS];
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) if (t0 + i < p.L) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
+    }
+    S A[V], H[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+    const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        const bool in = whole || t0 + i < p.L;
+        S s0[V];
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) s0[v] = S(0);
+            if ((m.start >> i) & 1) {
+                const int64_t s = seq_behind(p, t0 + i);
+                if (p.h0 && s < p.nseq) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) s0[v] = ((const S*)p.h0)[s * p.D + cl + v];
+                }
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            S rest = S(0);
+            if (in) {
+                decay<FORM, COUPLED, S>((S)rg[i].v[v], a[i][v], rest);
+                u[i][v] = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
+            } else { a[i][v] = S(1); u[i][v] = S(0); }
+            if constexpr (PACKED) {
+                if ((m.start >> i) & 1) u[i][v] += a[i][v] * s0[v];
+                if ((m.out >> i) & 1) u[i][v] = S(0);
+                if ((cuts >> i) & 1) { A[v] = S(0); H[v] = u[i][v]; } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + u[i][v]; }
+            } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + u[i][v]; }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) { sh.A[wave][lane * V + v] = A[v]; sh.H[wave][lane * V + v] = H[v]; }
+    if (lane == 0) sh.cut[wave] = cuts != 0;
+    S first[V], st[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) first[v] = (!PACKED && p.h0) ? ((const S*)p.h0)[b * p.D + cl + v] : S(0);
+    chain<S, V>(p, sh, c, k, first, st);
+    for (int w = 0; w < wave; ++w) {
+        const uint32_t q = sh.cut[w];
+#pragma unroll
+        for (int v = 0; v < V; ++v) st[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, st[v]);
+    }
+    if (p.ckpt && on && wave * TS % TTA == 0 && t0 / TTA < p.nckpt) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) ((S*)p.ckpt)[(b * p.nckpt + t0 / TTA) * p.D + ch + v] = st[v];
+    }
+    const int64_t ho = b * p.h_sb + t0 * p.h_st + ch;
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) st[v] = (PACKED && ((cuts >> i) & 1)) ? u[i][v] : a[i][v] * st[v] + u[i][v];
+        if (on && (whole || t0 + i < p.L)) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o.v[v] = (T)st[v];
+            *(Pack<T, V>*)((T*)p.h + ho + i * p.h_st) = o;
+        }
+        if constexpr (PACKED) {
+            if ((m.end >> i) & 1) {
+                const int64_t s = seq_behind(p, t0 + i);
+                if (on && s < p.nseq) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) ((S*)p.h_final)[s * p.D + ch + v] = st[v];
+                }
+            }
+        }
+    }
+    if constexpr (PACKED) {                                   // a sequence without rows ends where it starts
+        for (int64_t s = (int64_t)k * NW + wave; s < p.nseq; s += (int64_t)p.ntiles * NW)
+            if (offset_at(p, s + 1) <= offset_at(p, s) && on) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) ((S*)p.h_final)[s * p.D + ch + v] = p.h0 ? ((const S*)p.h0)[s * p.D + ch + v] : S(0);
+            }
+    } else if (on && k == p.ntiles - 1 && (p.L ? (t0 <= p.L - 1 && t0 + TS > p.L - 1) : wave == 0)) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) ((S*)p.h_final)[b * p.D + ch + v] = st[v];
+    }
+}
+
+// ---- adjoint ------------------------------------------------------------------------------------------------------------------------------------------------------
+
+template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
+__global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Args p) {
+    __shared__ Lds<S, V> sh;
+    constexpr int CW = 64 * V, TS = TSA;
+    constexpr bool REST = COUPLED || FORM == 2;
+    int64_t c; int k;
+    take(p, sh, c, k);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int64_t b = c / p.ncg, cg = c % p.ncg, ch = cg * CW + lane * V;
+    const bool on = ch < p.D;
+    const int64_t cl = on ? ch : 0;
+    const int tile = p.ntiles - 1 - k;                        // the scan runs from the end: position 0 is the last tile
+    const int64_t t0 = (int64_t)tile * TTA + wave * TS;
+    const int64_t xo = b * p.x_sb + t0 * p.x_st + cl, go = b * p.g_sb + t0 * p.g_st + cl, dho = b * p.dh_sb + t0 * p.dh_st + cl;
+    const bool whole = t0 + TS <= p.L;
+    Pack<T, V> rx[TS], rd[TS]; Pack<TG, V> rg[TS];
+    if (whole) {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
+    } else {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) if (t0 + i < p.L) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
+    }
+    if (whole && p.dh) {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) rd[i] = read<T, V>(p.dh, dho + i * p.dh_st);
+    } else {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+            if (p.dh && t0 + i < p.L) rd[i] = read<T, V>(p.dh, dho + i * p.dh_st);
+            else {
+#pragma unroll
+                for (int v = 0; v < V; ++v) rd[i].v[v] = (T)S(0);
+            }
+        }
+    }
+    Marks m{0, 0, 0};
+    if constexpr (PACKED) m = marks_of<TS>(p, t0);
+    const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
+    S a[TS][V], before[TS][V];                                // a of each row; first its b, then the state before it
+    S A[V], H[V], F[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+    auto at_seq = [&](const void* rows, int i, int v) -> S {  // row of the sequence that row i belongs to, in h0 or dh_final
+        const int64_t s = seq_behind(p, t0 + i);
+        return rows && s < p.nseq ? ((const S*)rows)[s * p.D + cl + v] : S(0);
+    };
+    // the rows' forward map, for the states
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        const bool in = whole || t0 + i < p.L;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            S rest = S(0), bb = S(0);
+            if (in) {
+                decay<FORM, COUPLED, S>((S)rg[i].v[v], a[i][v], rest);
+                bb = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
+            } else a[i][v] = S(1);
+            if constexpr (PACKED) { if ((m.out >> i) & 1) bb = S(0); }
+            before[i][v] = bb;
+            if constexpr (PACKED) {
+                if ((m.start >> i) & 1) bb += a[i][v] * at_seq(p.h0, i, v);
+                if ((cuts >> i) & 1) { A[v] = S(0); H[v] = bb; } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + bb; }
+            } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + bb; }
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) { sh.A[wave][lane * V + v] = A[v]; sh.H[wave][lane * V + v] = H[v]; }
+    if (lane == 0) sh.cut[wave] = cuts != 0;
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < V; ++v) F[v] = ((const S*)p.ckpt)[(b * p.nckpt + tile) * p.D + cl + v];
+    for (int w = 0; w < wave; ++w) {
+        const uint32_t q = sh.cut[w];
+#pragma unroll
+        for (int v = 0; v < V; ++v) F[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, F[v]);
+    }
+    __syncthreads();
+    // the cotangent of a row's state from outside the recurrence (a sequence's last row also feeds its final state); nothing in a row of no sequence
+    auto cot = [&](int i, int v) -> S {
+        S d = (S)rd[i].v[v];
+        if constexpr (PACKED) {
+            if ((m.out >> i) & 1) d = S(0);
+            if ((m.end >> i) & 1) d += at_seq(p.dh_final, i, v);
+        }
+        return d;
+    };
+    // the rows' reverse map R -> A R + H with the same product A
+#pragma unroll
+    for (int v = 0; v < V; ++v) H[v] = S(0);
+#pragma unroll
+    for (int i = TS - 1; i >= 0; --i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) { const S d = cot(i, v); H[v] = (PACKED && ((cuts >> i) & 1)) ? S(0) : a[i][v] * (d + H[v]); }
+    }
+    const int rw = NW - 1 - wave;                             // the piece's place in scan order
+#pragma unroll
+    for (int v = 0; v < V; ++v) { sh.A[rw][lane * V + v] = A[v]; sh.H[rw][lane * V + v] = H[v]; }
+    if (lane == 0) sh.cut[rw] = cuts != 0;
+    S first[V], R[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) first[v] = (!PACKED && p.dh_final) ? ((const S*)p.dh_final)[b * p.D + cl + v] : S(0);
+    chain<S, V>(p, sh, c, k, first, R);
+    for (int w = 0; w < rw; ++w) {
+        const uint32_t q = sh.cut[w];
+#pragma unroll
+        for (int v = 0; v < V; ++v) R[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, R[v]);
+    }
+    // the states before each row, then the rows from the last to the first
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (PACKED && ((m.start >> i) & 1)) F[v] = at_seq(p.h0, i, v);
+            const S bb = before[i][v];
+            before[i][v] = F[v];
+            F[v] = a[i][v] * F[v] + bb;
+            if (PACKED && ((m.out >> i) & 1)) F[v] = S(0);
+        }
+    }
+    const int64_t dxo = b * p.dx_sb + t0 * p.dx_st + ch, dgo = b * p.dg_sb + t0 * p.dg_st + ch;
+#pragma unroll
+    for (int i = TS - 1; i >= 0; --i) {
+        const bool in = whole || t0 + i < p.L;
+        Pack<T, V> ox; Pack<TG, V> og;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const S G = cot(i, v) + R[v];
+            S aa = a[i][v], rest = S(1), x = S(0);
+            if (in) {
+                if constexpr (REST) decay<FORM, true, S>((S)rg[i].v[v], aa, rest);
+                if constexpr (COUPLED) x = (S)rx[i].v[v];
+            }
+            S da = G * (before[i][v] - x);
+            if constexpr (FORM == 1) da *= a[i][v];
+            if constexpr (FORM == 2) da *= a[i][v] * rest;
+            S dx = COUPLED ? G * rest : G;
+            R[v] = a[i][v] * G;
+            if (PACKED && ((m.out >> i) & 1)) { da = S(0); dx = S(0); R[v] = S(0); }
+            ox.v[v] = (T)dx; og.v[v] = (TG)da;
+        }
+        if (on && in) {
+            if (p.dx) *(Pack<T, V>*)((T*)p.dx + dxo + i * p.dx_st) = ox;
+            if (p.dgate) *(Pack<TG, V>*)((TG*)p.dgate + dgo + i * p.dg_st) = og;
+        }
+        if constexpr (PACKED) {
+            if ((m.start >> i) & 1) {
+                const int64_t s = seq_behind(p, t0 + i);
+                if (on && p.dh0 && s < p.nseq) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) ((S*)p.dh0)[s * p.D + ch + v] = R[v];
+                }
+#pragma unroll
+                for (int v = 0; v < V; ++v) R[v] = S(0);
+            }
+        }
+    }
+    if constexpr (PACKED) {
+        for (int64_t s = (int64_t)k * NW + wave; s < p.nseq; s += (int64_t)p.ntiles * NW)
+            if (offset_at(p, s + 1) <= offset_at(p, s) && on && p.dh0) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) ((S*)p.dh0)[s * p.D + ch + v] = p.dh_final ? ((const S*)p.dh_final)[s * p.D + ch + v] : S(0);
+            }
+    } else if (on && tile == 0 && wave == 0 && p.dh0) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) ((S*)p.dh0)[b * p.D + ch + v] = R[v];
+    }
+}
+
+// ---- single step --------------------------------------------------------------------------------------------------------------------------------------------------
+// One row per sequence: state[slot] = a state[slot] + b, h = the new state.  Rows that name the same slot are steps of one sequence in the order of the rows: the first of them
+// takes all, so no two workgroups touch a state.  A slot outside [0, nslots) (-1 pads a batch) has no state: its h is zero.
+struct StepArgs {
+    const void *x, *gate, *slots;
+    void *state, *h;
+    int64_t x_s, g_s, st_s, h_s, B, D, nslots;
+    int32_t slots64;
+};
+constexpr int NS = 256;
+template <class T, class TG, class S, int V, int FORM, bool COUPLED>
+__global__ void __launch_bounds__(NS) k_step(const StepArgs p, int ncg) {
+    const int64_t r = blockIdx.x / (uint32_t)ncg, ch = ((int64_t)(blockIdx.x % (uint32_t)ncg) * NS + threadIdx.x) * V;
+    const bool on = ch < p.D;
+    auto slot_of = [&](int64_t i) -> int64_t { return p.slots64 ? ((const int64_t*)p.slots)[i] : (int64_t)((const int32_t*)p.slots)[i]; };
+    const int64_t slot = p.slots ? slot_of(r) : r;
+    if (slot < 0 || slot >= p.nslots) {
+        if (on) {
+            Pack<T, V> o;
+#pragma unroll
+            for (int v = 0; v < V; ++v) o.v[v] = (T)S(0);
+            *(Pack<T, V>*)((T*)p.h + r * p.h_s + ch) = o;
+        }
+        return;
+    }
+    bool more = false;
+    if (p.slots) {
+        bool earlier = false, later = false;
+        for (int64_t i = threadIdx.x; i < p.B; i += NS) if (i != r && slot_of(i) == slot) { if (i < r) earlier = true; else later = true; }
+        if (__syncthreads_or(earlier)) return;
+        more = __syncthreads_or(later);
+    }
+    if (!on) return;
+    S st[V];
+    S* sp = (S*)p.state + slot * p.st_s + ch;
+    {
+        const Pack<S, V> q = *(const Pack<S, V>*)sp;
+#pragma unroll
+        for (int v = 0; v < V; ++v) st[v] = q.v[v];
+    }
+    for (int64_t i = r; i < p.B; ++i) {
+        if (i != r) { if (!more) break; if (slot_of(i) != slot) continue; }
+        const Pack<T, V> x = read<T, V>(p.x, i * p.x_s + ch);
+        const Pack<TG, V> g = read<TG, V>(p.gate, i * p.g_s + ch);
+        Pack<T, V> o;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            S a, rest = S(0);
+            decay<FORM, COUPLED, S>((S)g.v[v], a, rest);
+            st[v] = a * st[v] + (COUPLED ? rest * (S)x.v[v] : (S)x.v[v]);
+            o.v[v] = (T)st[v];
+        }
+        *(Pack<T, V>*)((T*)p.h + i * p.h_s + ch) = o;
+    }
+    Pack<S, V> q;
+#pragma unroll
+    for (int v = 0; v < V; ++v) q.v[v] = st[v];
+    *(Pack<S, V>*)sp = q;
+}
+
+// one launch per (types, vector width, form, coupled, packed); translation units instantiate these (hipadj_tu_recurrence.hip)
+enum { PAIR_F64 = 0, PAIR_F32, PAIR_BF16, PAIR_BF16_F32, PAIR_F16, PAIR_F16_F32 };     // (x, gate)
+template <int PAIR> struct Types;
+template <> struct Types<PAIR_F64> { typedef double T, TG, S; static constexpr int V = 1; };
+template <> struct Types<PAIR_F32> { typedef float T, TG, S; static constexpr int V = 1; };
+template <> struct Types<PAIR_BF16> { typedef bf16 T, TG; typedef float S; static constexpr int V = 2; };
+template <> struct Types<PAIR_BF16_F32> { typedef bf16 T; typedef float TG, S; static constexpr int V = 2; };
+template <> struct Types<PAIR_F16> { typedef f16 T, TG; typedef float S; static constexpr int V = 2; };
+template <> struct Types<PAIR_F16_F32> { typedef f16 T; typedef float TG, S; static constexpr int V = 2; };
+
+template <int PAIR> void launch(const Args& a, bool adjoint, bool wide, int form, bool coupled, bool packed, hipStream_t stream);
+template <int PAIR> void launch_step(const StepArgs& a, bool wide, int form, bool coupled, hipStream_t stream);
+
+}  // namespace rec

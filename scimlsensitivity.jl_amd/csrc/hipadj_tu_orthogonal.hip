@@ -1,0 +1,139 @@
+// hipadj_tu_orthogonal.hip — the orthogonalised update: launches and C entry points.
+#include <algorithm>
+#include <cmath>
+#include <cstdio>
+#include "hipadj_ops.hpp"
+#include "hipadj_orthogonal.hpp"
+
+namespace orth {
+
+struct Plan { Mat q; bool split; int64_t bytes; };
+
+static int64_t padded(int64_t v) { return (v + PADDED - 1) / PADDED * PADDED; }
+
+// One F16 term a factor where BF16 rounds the output anyway and the matrix is large enough for the products to be what it costs; see hipadj_orthogonal.hpp for the error
+static bool one_term(const hipadj_orthogonal* o) { return o->dtype == HIPADJ_BF16 && std::min(o->rows, o->cols) >= 256; }
+
+static Plan plan_of(const hipadj_orthogonal* o, char* base) {
+    Plan p;
+    Mat& q = p.q;
+    q.flip = o->rows > o->cols;
+    q.m = std::min(o->rows, o->cols); q.n = std::max(o->rows, o->cols);
+    q.mp = padded(q.m); q.np = padded(q.n);
+    q.batch = o->batch;
+    p.split = !one_term(o);
+    int64_t at = 0;
+    auto take = [&](int64_t bytes) { char* r = base + at; at += (bytes + 255) / 256 * 256; return r; };
+    const int T = p.split ? 2 : 1;
+    q.x[1] = q.xt[0][1] = q.xt[1][1] = q.a[1] = q.b[1] = nullptr;
+    for (int t = 0; t < T; ++t) {
+        q.x[t] = (f16*)take(q.batch * q.mp * q.np * 2);
+        q.xt[0][t] = (f16*)take(q.batch * q.mp * q.np * 2);
+        q.xt[1][t] = (f16*)take(q.batch * q.mp * q.np * 2);
+        q.a[t] = (f16*)take(q.batch * q.mp * q.mp * 2);
+        q.b[t] = (f16*)take(q.batch * q.mp * q.mp * 2);
+    }
+    q.master = (float*)take(q.batch * q.mp * q.np * 4);
+    q.partial = (double*)take(q.batch * NORM_BLOCKS * 8);
+    p.bytes = at;
+    return p;
+}
+
+template <class T, int BT, int EPI, bool SPLIT> static void product(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
+    const int64_t ti = g.M / BT, tj = g.N / BT;
+    const dim3 grid = EPI == GRAM || EPI == POLY ? dim3((uint32_t)(ti * (ti + 1) / 2), 1, (uint32_t)q.batch) : dim3((uint32_t)tj, (uint32_t)ti, (uint32_t)q.batch);
+    k_product<T, BT, EPI, SPLIT><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
+}
+
+template <class T, int BT, bool SPLIT> static void iterate(const hipadj_orthogonal* o, const Mat& q, const Io<T>& io, hipStream_t s) {
+    k_norm<T><<<dim3(NORM_BLOCKS, (uint32_t)q.batch), dim3(256), 0, s>>>(io, q.partial);
+    k_start<T, SPLIT><<<dim3((uint32_t)(q.np / 64), (uint32_t)(q.mp / 64), (uint32_t)q.batch), dim3(256), 0, s>>>(io, q);
+    const int64_t smm = q.mp * q.mp, smn = q.mp * q.np;
+    auto rounded = [&](int step) { return !SPLIT && step >= o->steps - 2; };
+    for (int step = 0; step < o->steps; ++step) {
+        const double* c = o->coefficients + 3 * step;
+        const int from = step & 1, to = 1 - from;
+        Product g{};
+        g.c0 = (float)c[0]; g.c1 = (float)c[1]; g.c2 = (float)c[2];
+        g.P[0] = g.Q[0] = q.x[0]; g.P[1] = g.Q[1] = q.x[1]; g.sP = g.sQ = smn; g.K = q.np; g.M = g.N = q.mp;
+        product<T, BT, GRAM, SPLIT>(g, q, io, from, to, s);
+        g.P[0] = g.Q[0] = q.a[0]; g.P[1] = g.Q[1] = q.a[1]; g.sP = g.sQ = smm; g.K = q.mp;
+        product<T, BT, POLY, SPLIT>(g, q, io, from, to, s);
+        g.P[0] = q.b[0]; g.P[1] = q.b[1]; g.sP = smm;
+        g.Q[0] = q.xt[from][0]; g.Q[1] = q.xt[from][1]; g.sQ = smn; g.N = q.np;
+        g.rounded = rounded(step); g.keep = !rounded(step + 1);
+        if (step + 1 < o->steps) product<T, BT, APPLY, SPLIT>(g, q, io, from, to, s);
+        else product<T, BT, LAST, SPLIT>(g, q, io, from, to, s);
+    }
+}
+
+template <class T> static void run(const hipadj_orthogonal* o, const Plan& p, const void* grad, float* mom, void* out, hipStream_t s) {
+    Io<T> io;
+    io.grad = (const T*)grad; io.mom = mom; io.out = (T*)out; io.rows = o->rows; io.cols = o->cols;
+    io.g_b = o->grad_stride[0]; io.g_r = o->grad_stride[1]; io.m_b = o->momentum_stride[0]; io.m_r = o->momentum_stride[1]; io.o_b = o->out_stride[0]; io.o_r = o->out_stride[1];
+    io.beta = (float)o->beta; io.scale = (float)o->scale; io.nesterov = o->nesterov;
+    if (p.split) iterate<T, 128, true>(o, p.q, io, s);
+    else if constexpr (sizeof(T) == 2) iterate<T, 128, false>(o, p.q, io, s);
+}
+
+// How far the coefficients let the iteration grow: X starts with singular values in [0, 1], a step maps a bound s to the largest |c0 x + c1 x^3 + c2 x^5| on [0, s], reached at s or where
+// the derivative vanishes, and B has eigenvalues c1 y + c2 y^2, y <= s^2.  F16 holds 2^13 X up to 8 and 2^11 B up to 32.
+static bool grows(const hipadj_orthogonal* o, double& s, double& big) {
+    s = 1.0; big = 0.0;
+    for (int k = 0; k < o->steps; ++k) {
+        const double c0 = o->coefficients[3 * k], c1 = o->coefficients[3 * k + 1], c2 = o->coefficients[3 * k + 2];
+        auto p = [&](double x) { return std::fabs(x * (c0 + x * x * (c1 + x * x * c2))); };
+        auto b = [&](double y) { return std::fabs(y * (c1 + y * c2)); };
+        double most = p(s), mb = b(s * s);
+        const double disc = 9 * c1 * c1 - 20 * c0 * c2;
+        if (disc >= 0)
+            for (int sign = -1; sign <= 1; sign += 2) {
+                const double d = -3 * c1 + sign * std::sqrt(disc), y = c2 != 0 ? d / (10 * c2) : (c1 != 0 ? -c0 / (3 * c1) : -1.0);
+                if (y > 0 && y < s * s) most = std::max(most, p(std::sqrt(y)));
+            }
+        if (c2 != 0 && -c1 / (2 * c2) > 0 && -c1 / (2 * c2) < s * s) mb = std::max(mb, b(-c1 / (2 * c2)));
+        big = std::max(big, mb);
+        s = most;
+        if (s > 6.0 || big > 24.0) return true;
+    }
+    return false;
+}
+
+static int check(const hipadj_orthogonal* o) {
+    if (!o || o->struct_size != sizeof(hipadj_orthogonal)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonal.struct_size does not match this library");
+    if (o->dtype != HIPADJ_F32 && o->dtype != HIPADJ_BF16 && o->dtype != HIPADJ_F16) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: matrices are F32, BF16 or F16");
+    if (o->batch < 0 || o->rows < 0 || o->cols < 0) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: negative size");
+    if (o->steps < 1 || o->steps > 64 || !o->coefficients) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: 1 to 64 steps with three coefficients each, got %d", o->steps);
+    for (int i = 0; i < 3 * o->steps; ++i)
+        if (!(std::fabs(o->coefficients[i]) <= 32.0)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: coefficients within +-32, got %g", o->coefficients[i]);
+    double s, big;
+    if (grows(o, s, big)) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: with these coefficients singular values can grow to %.3g (at most 6) and c1 A + c2 A A to %.3g (at most 24)", s, big);
+    if (!std::isfinite(o->beta) || !std::isfinite(o->scale)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: beta and scale must be finite");
+    if (std::max(o->rows, o->cols) > 65536 || std::min(o->rows, o->cols) > 32768 || o->batch > 65535)
+        return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: at most 65535 matrices with sides of at most 32768 and 65536");
+    return HIPADJ_OK;
+}
+
+}  // namespace orth
+
+extern "C" int hipadj_orthogonalized_update_size(const hipadj_orthogonal* o, int64_t* workspace_bytes) {
+    const int rc = orth::check(o);
+    if (rc != HIPADJ_OK) return rc;
+    if (workspace_bytes) *workspace_bytes = orth::plan_of(o, nullptr).bytes;
+    return HIPADJ_OK;
+}
+
+extern "C" int hipadj_orthogonalized_update_dev(const hipadj_orthogonal* o, const void* grad, float* momentum, void* out, void* workspace, void* stream) {
+    const int rc = orth::check(o);
+    if (rc != HIPADJ_OK) return rc;
+    if (o->batch == 0 || o->rows == 0 || o->cols == 0) return HIPADJ_OK;
+    if (!grad || !out || !workspace || (uintptr_t)workspace % 256) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonalized_update_dev: grad, out and a 256-byte aligned workspace are required");
+    const orth::Plan p = orth::plan_of(o, (char*)workspace);
+    OpsDevice dev(o->device);
+    if (dev.rc != HIPADJ_OK) return dev.rc;
+    hipStream_t s = (hipStream_t)stream;
+    if (o->dtype == HIPADJ_F32) orth::run<float>(o, p, grad, momentum, out, s);
+    else if (o->dtype == HIPADJ_BF16) orth::run<orth::bf16>(o, p, grad, momentum, out, s);
+    else orth::run<orth::f16>(o, p, grad, momentum, out, s);
+    return ops_launched("orthogonalized update");
+}

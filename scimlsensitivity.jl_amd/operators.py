@@ -1,0 +1,272 @@
+"""Operators of sequence models on torch device tensors, next to the solves: the gated linear recurrence with its adjoint and its single step, and the
+orthogonalised update of weight matrices (include/hipadj.h: hipadj_recurrence*, hipadj_orthogonalized_update*).
+
+torch is used for device memory and streams only: a call runs on torch's current stream of its tensors' device, its workspace comes from torch's allocator on that
+stream, nothing is kept between calls, and nothing waits for the device (so every call can be captured into a graph)."""
+import ctypes as C
+
+from . import _lib
+from ._lib import HipadjError, HipadjOrthogonal, HipadjRecurrence
+
+GATES = {"decay": 0, "log": 1, "sigmoid": 2}
+_DTYPES = None
+
+
+def _torch():
+    global _DTYPES
+    import torch
+    if _DTYPES is None:
+        _DTYPES = {torch.float64: 0, torch.float32: 1, torch.bfloat16: 2, torch.float16: 3}
+    return torch
+
+
+def _check(rc):
+    if rc != _lib.OK:
+        raise HipadjError(rc, _lib.load().hipadj_last_error(None).decode())
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(torch, device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on(name, t, like, dtype=None, shape=None):
+    if t.device != like.device:
+        raise ValueError(f"{name} lives on {t.device}, x on {like.device}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _rows(t):
+    """t with channels next to each other: as it is, or a copy."""
+    return t if t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _gate_types(torch, x, gate, form):
+    if not x.is_cuda:
+        raise ValueError("x must be a GPU tensor: there is no CPU fallback")
+    if form not in GATES:
+        raise ValueError(f"form must be one of {sorted(GATES)}, got {form!r}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"x must be float64, float32, bfloat16 or float16, got {x.dtype}")
+    if gate.dtype != x.dtype and not (gate.dtype == torch.float32 and x.dtype in (torch.bfloat16, torch.float16)):
+        raise ValueError(f"gate must have x's type ({x.dtype}), or float32 next to bfloat16 / float16; got {gate.dtype}")
+    _on("gate", gate, x, shape=x.shape)
+    return torch.float64 if x.dtype == torch.float64 else torch.float32
+
+
+class RecurrenceSolution:
+    """What recurrence_solve returns: h [like x], h_final [rows][channels], and what recurrence_adjoint needs of the forward pass (x, the gate and h0 by
+    reference — they must not change before the adjoint — and the states at the checkpoints)."""
+    __slots__ = ("h", "h_final", "x", "gate", "h0", "offsets", "form", "coupled", "_checkpoints", "_config", "_workspace_bytes", "_state_type", "_final_shape")
+
+
+def _strides(t, packed):
+    """(batch, time) strides; a batch of one has none."""
+    if packed:
+        return (0, t.stride(0))
+    return (t.stride(0) if t.shape[0] > 1 else 0, t.stride(1) if t.shape[1] > 1 else 0)
+
+
+def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=None, adjoint=True):
+    """The gated linear recurrence h_t = a_t h_{t-1} + b_t of every channel: a = gate ("decay"), exp(gate) ("log") or sigmoid(gate) ("sigmoid"); b = x, or
+    (1 - a) x when coupled — with form="log" and gate = -r dt that is the diagonal system h' = r (x - h) stepped exactly.
+
+    x, gate [batch][length][channels] (any batch and time strides), h0 [batch][channels] (None: zeros); or packed sequences: x, gate [rows][channels] and offsets
+    [nseq + 1] (int32 / int64 on the same device, ascending), h0 [nseq][channels].  Types: float64, float32, bfloat16, float16; the gate may be float32 next to the
+    16-bit ones; h0 and h_final are float64 for float64 and float32 otherwise.  Rows of no sequence get h = 0.
+    adjoint=False leaves out the checkpoints that recurrence_adjoint reads.  Returns a RecurrenceSolution."""
+    torch = _torch()
+    packed = offsets is not None
+    if x.dim() != (2 if packed else 3):
+        raise ValueError(f"x must be {'[rows][channels]' if packed else '[batch][length][channels]'}, got shape {tuple(x.shape)}")
+    wide = _gate_types(torch, x, gate, form)
+    x, gate = _rows(x), _rows(gate)
+    batch, length, channels = (1, *x.shape) if packed else x.shape
+    nseq = 0
+    if packed:
+        _on("offsets", offsets, x)
+        if offsets.dim() != 1 or offsets.numel() < 2 or offsets.dtype not in (torch.int32, torch.int64):
+            raise ValueError("offsets must be int32 or int64 [nseq + 1] with at least one sequence")
+        offsets = offsets.contiguous()
+        nseq = offsets.numel() - 1
+    rows = nseq or batch
+    if h0 is not None:
+        h0 = _on("h0", h0, x, wide, (rows, channels)).contiguous()
+    r = HipadjRecurrence()
+    r.struct_size, r.device, r.dtype, r.gate_dtype = C.sizeof(HipadjRecurrence), x.device.index, _DTYPES[x.dtype], _DTYPES[gate.dtype]
+    r.gate, r.coupled, r.batch, r.length, r.channels, r.nseq = GATES[form], int(bool(coupled)), batch, length, channels, nseq
+    if packed:
+        r.offsets, r.offsets_bits = offsets.data_ptr(), 64 if offsets.dtype == torch.int64 else 32
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    r.x_stride[:], r.gate_stride[:], r.h_stride[:] = _strides(x, packed), _strides(gate, packed), _strides(h, packed)
+    L = _lib.load()
+    ck, ws = C.c_int64(), C.c_int64()
+    _check(L.hipadj_recurrence_sizes(C.byref(r), C.byref(ck), C.byref(ws)))
+    sol = RecurrenceSolution()
+    sol.h, sol.h_final = h, torch.empty((rows, channels), dtype=wide, device=x.device)
+    sol._checkpoints = torch.empty(ck.value, dtype=torch.uint8, device=x.device) if adjoint else None
+    work = torch.empty(ws.value, dtype=torch.uint8, device=x.device) if ws.value else None
+    _check(L.hipadj_recurrence_forward_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(h0), _ptr(h), _ptr(sol.h_final), _ptr(sol._checkpoints), _ptr(work), _stream(torch, x.device)))
+    sol.x, sol.gate, sol.h0, sol.offsets, sol.form, sol.coupled = x, gate, h0, offsets, form, bool(coupled)
+    sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape = r, ws.value, wide, (rows, channels)
+    return sol
+
+
+def recurrence_adjoint(sol, dh=None, dh_final=None, *, need=(True, True, True)):
+    """(dx, dgate, dh0): the gradients of sum(dh * h) + sum(dh_final * h_final) with respect to x, gate and h0 (also for h0=None: of the zeros), each of its
+    argument's type; dh [like h], dh_final [like h_final], None = zeros.  need: which of the three to compute (the others are None)."""
+    torch = _torch()
+    if sol._checkpoints is None:
+        raise ValueError("the solution was computed with adjoint=False: it has no checkpoints")
+    x, gate, packed = sol.x, sol.gate, sol.offsets is not None
+    r = HipadjRecurrence.from_buffer_copy(sol._config)
+    if dh is not None:
+        dh = _rows(_on("dh", dh, x, x.dtype, x.shape))
+        r.dh_stride[:] = _strides(dh, packed)
+    if dh_final is not None:
+        dh_final = _on("dh_final", dh_final, x, sol._state_type, sol._final_shape).contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    dgate = torch.empty(gate.shape, dtype=gate.dtype, device=x.device) if need[1] else None
+    dh0 = torch.empty(sol._final_shape, dtype=sol._state_type, device=x.device) if need[2] else None
+    if dx is not None:
+        r.dx_stride[:] = _strides(dx, packed)
+    if dgate is not None:
+        r.dgate_stride[:] = _strides(dgate, packed)
+    work = torch.empty(sol._workspace_bytes, dtype=torch.uint8, device=x.device) if sol._workspace_bytes else None
+    _check(_lib.load().hipadj_recurrence_adjoint_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(sol.h0), _ptr(sol._checkpoints), _ptr(dh), _ptr(dh_final), _ptr(dx), _ptr(dgate), _ptr(dh0),
+                                                     _ptr(work), _stream(torch, x.device)))
+    return dx, dgate, dh0
+
+
+_function = None
+
+
+def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=None):
+    """(h, h_final) of the gated linear recurrence (recurrence_solve), differentiable by torch's autograd with respect to x, gate and h0; first derivatives."""
+    global _function
+    torch = _torch()
+    if _function is None:
+        class GatedRecurrence(torch.autograd.Function):
+            @staticmethod
+            def forward(ctx, x, gate, h0, form, coupled, offsets):
+                want = any(ctx.needs_input_grad[:3])
+                sol = recurrence_solve(x, gate, h0, form=form, coupled=coupled, offsets=offsets, adjoint=want)
+                if want:
+                    ctx.save_for_backward(sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints)      # versions are checked: a changed input is an error, not a wrong gradient
+                    ctx.rest = (sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape)
+                    ctx.set_materialize_grads(False)
+                return sol.h, sol.h_final
+
+            @staticmethod
+            @torch.autograd.function.once_differentiable
+            def backward(ctx, dh, dh_final):
+                sol = RecurrenceSolution()
+                sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints = ctx.saved_tensors
+                sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape = ctx.rest
+                dx, dgate, dh0 = recurrence_adjoint(sol, dh, dh_final, need=ctx.needs_input_grad[:3])
+                return dx, dgate, dh0, None, None, None
+        _function = GatedRecurrence
+    return _function.apply(x, gate, h0, form, coupled, offsets)
+
+
+def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=None):
+    """One step of running sequences: state[slots[i]] <- a state[slots[i]] + b in place, and h[i] = the new state in x's type.  x, gate [batch][channels]; state
+    [nslots][channels] float32 (float64 for float64); slots int32 / int64 [batch] or None (row i has state i).  A slot outside the states (-1) pads the batch: h[i] = 0.
+    Rows with the same slot are consecutive steps of that state in row order."""
+    torch = _torch()
+    if x.dim() != 2:
+        raise ValueError(f"x must be [batch][channels], got shape {tuple(x.shape)}")
+    wide = _gate_types(torch, x, gate, form)
+    if state.device != x.device or state.dtype != wide or state.dim() != 2 or state.shape[1] != x.shape[1] or (state.shape[1] > 1 and state.stride(1) != 1):
+        raise ValueError(f"state must be {wide} [nslots][{x.shape[1]}] on {x.device} with neighbouring channels, got {state.dtype} {tuple(state.shape)} on {state.device}")
+    if state.shape[0] > 1 and abs(state.stride(0)) < state.shape[1]:
+        raise ValueError("the rows of state overlap")
+    if slots is not None:
+        if slots.device != x.device or slots.dtype not in (torch.int32, torch.int64) or tuple(slots.shape) != (x.shape[0],):
+            raise ValueError(f"slots must be int32 or int64 [{x.shape[0]}] on {x.device}")
+        slots = slots.contiguous()
+    elif state.shape[0] < x.shape[0]:
+        raise ValueError(f"{x.shape[0]} rows without slots need as many states, got {state.shape[0]}")
+    x, gate = _rows(x), _rows(gate)
+    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _check(_lib.load().hipadj_recurrence_step_dev(x.device.index, _DTYPES[x.dtype], _DTYPES[gate.dtype], GATES[form], bool(coupled), x.shape[0], x.shape[1], x.data_ptr(), x.stride(0),
+                                                  gate.data_ptr(), gate.stride(0), state.data_ptr(), state.stride(0), state.shape[0], _ptr(slots),
+                                                  64 if slots is not None and slots.dtype == torch.int64 else 32, h.data_ptr(), h.stride(0), _stream(torch, x.device)))
+    return h
+
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)      # the usual quintic: steep at zero, singular values end in 0.7 ... 1.2 (K. Jordan, Muon, 2024)
+
+
+def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, steps=5, coefficients=NEWTON_SCHULZ, scale=1.0, out=None):
+    """The orthogonalised update of weight matrices: momentum <- beta momentum + grad (in place, float32, like grad; None: no momentum), u = grad + beta momentum
+    (nesterov) or momentum, X = u / (|u| + 1e-7), `steps` times X <- c0 X + c1 A X + c2 A A X with A = X X', and scale X is returned in grad's type.
+
+    grad [..., rows, cols] float32, bfloat16 or float16: every matrix of the leading dimensions by itself (heads, layers); row-major or its transpose.
+    coefficients: three numbers, or three for each step.  out: where to write (like grad; grad itself is allowed).  For weights W [out, in] the usual step is
+    W -= lr * orthogonalized_update(dW, m, scale=max(1, out / in) ** 0.5)."""
+    torch = _torch()
+    if not grad.is_cuda:
+        raise ValueError("grad must be a GPU tensor: there is no CPU fallback")
+    if grad.dim() < 2:
+        raise ValueError(f"grad must be [..., rows, cols], got shape {tuple(grad.shape)}")
+    if grad.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError(f"grad must be float32, bfloat16 or float16, got {grad.dtype}")
+    for name, t, dt in (("momentum", momentum, torch.float32), ("out", out, grad.dtype)):
+        if t is not None:
+            _on(name, t, grad, dt, grad.shape)
+    co = [float(c) for row in coefficients for c in row] if len(coefficients) and not isinstance(coefficients[0], (int, float)) else [float(c) for c in coefficients] * int(steps)
+    if len(co) != 3 * int(steps):
+        raise ValueError(f"coefficients: three numbers, or three for each of the {steps} steps")
+
+    def matrices(t):       # [batch, rows, cols] with one stride between matrices; None where t's memory does not allow it
+        if t.dim() == 2:
+            return t.unsqueeze(0)
+        try:
+            return t.view(-1, *t.shape[-2:]) if t.dim() > 3 else t
+        except RuntimeError:
+            return None
+
+    def own(t):            # written in place: no two elements in one place
+        return t.numel() == 0 or all(s > 0 or n == 1 for s, n in zip(t.stride(), t.shape))
+
+    given_out = out
+    if out is None:
+        out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if grad.stride(-1) == 1 or grad.stride(-2) != 1 else \
+            torch.empty((*grad.shape[:-2], grad.shape[-1], grad.shape[-2]), dtype=grad.dtype, device=grad.device).transpose(-1, -2)
+    g, m, o = matrices(grad), None if momentum is None else matrices(momentum), matrices(out)
+    if g is None:
+        g = matrices(grad.contiguous())
+    if (momentum is not None and (m is None or not own(m))) or o is None or not own(o):
+        raise ValueError("momentum and out are written in place: their matrices must lie at one stride from each other and not overlap")
+    # one order for all: columns next to each other, or the transposes (the iteration commutes with transposition)
+    row_major = lambda t: t.shape[-1] <= 1 or t.stride(-1) == 1       # noqa: E731
+    written = [t for t in (m, o) if t is not None]
+    if not all(row_major(t) for t in written):
+        if not all(row_major(t.transpose(-1, -2)) for t in written):
+            raise ValueError("momentum and out must both be row-major or both be column-major")
+        g, o, m = g.transpose(-1, -2), o.transpose(-1, -2), None if m is None else m.transpose(-1, -2)
+    if not row_major(g):
+        g = g.contiguous()
+    q = HipadjOrthogonal()
+    q.struct_size, q.device, q.dtype, q.steps, q.nesterov = C.sizeof(HipadjOrthogonal), grad.device.index, _DTYPES[grad.dtype], int(steps), int(bool(nesterov))
+    q.batch, q.rows, q.cols = g.shape
+    q.grad_stride[:], q.out_stride[:] = (g.stride(0), g.stride(1)), (o.stride(0), o.stride(1))
+    if m is not None:
+        q.momentum_stride[:] = (m.stride(0), m.stride(1))
+    q.beta, q.scale = float(beta), float(scale)
+    co = (C.c_double * len(co))(*co)
+    q.coefficients = C.cast(co, C.POINTER(C.c_double))
+    L = _lib.load()
+    ws = C.c_int64()
+    _check(L.hipadj_orthogonalized_update_size(C.byref(q), C.byref(ws)))
+    work = torch.empty(ws.value, dtype=torch.uint8, device=grad.device)
+    _check(L.hipadj_orthogonalized_update_dev(C.byref(q), _ptr(g), _ptr(m), _ptr(o), _ptr(work), _stream(torch, grad.device)))
+    return given_out if given_out is not None else out
