@@ -27,7 +27,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float SX = 8192.f, SA = 2048.f;     // X and A, B are stored times these
-constexpr int BK = 64;                        // depth of a stage: a row of it is 128 bytes, eight 16-byte chunks
+constexpr int BK = 32;                        // depth of a stage: a row of it is 64 bytes, four 16-byte chunks
 constexpr int PADDED = 128;                   // sides are padded with zeros to multiples of this (the smaller tile), so the products have no edges
 
 struct Mat {                                  // one batch of matrices and the workspace it is computed in
@@ -36,9 +36,10 @@ struct Mat {                                  // one batch of matrices and the w
     bool flip;                                // X is the transpose of the caller's matrix
     f16 *x[2], *xt[2][2], *a[2], *b[2];       // [term]: x [batch][mp][np]; xt[buffer][term] [batch][np][mp]; a, b [batch][mp][mp]
     float* master;                            // 2^13 X in F32, transposed [batch][np][mp]
-    double* partial;                          // [batch][NORM_BLOCKS]
+    double* partial;                          // [batch][nblocks]
+    int nblocks;
 };
-constexpr int NORM_BLOCKS = 64;
+constexpr int NORM_BLOCKS = 1024;             // at most; Mat::nblocks of them
 
 // ---- gradient, momentum, norm -------------------------------------------------------------------------------------------------------------------------------------------
 template <class T> struct Io {
@@ -46,6 +47,7 @@ template <class T> struct Io {
     int64_t rows, cols, g_b, g_r, m_b, m_r, o_b, o_r;
     float beta, scale;
     int nesterov;
+    bool vec;                                 // rows of out start on multiples of four elements
 };
 template <class T> __device__ inline float moved(const Io<T>& io, int64_t b, int64_t r, int64_t c, bool update) {
     const float g = (float)io.grad[b * io.g_b + r * io.g_r + c];
@@ -64,15 +66,40 @@ __device__ inline double block_sum(double v) {       // 256 threads, fixed order
     return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-template <class T> __global__ void __launch_bounds__(256) k_norm(const Io<T> io, double* partial) {
-    const int64_t b = blockIdx.y, count = io.rows * io.cols;
+// Momentum and the partial sums of |u|^2.  A workgroup takes stretches of NORM_SPAN neighbouring elements (host side: matrices without gaps count as one row), 8 a thread with one
+// request where rows start on 16 bytes.  Reads 2 or 4 + 4 bytes an element, writes 4: memory-bound.
+constexpr int NORM_SPAN = 2048;
+template <class T> __global__ void __launch_bounds__(256) k_norm(const Io<T> io, int64_t rows, int64_t cols, bool vec, double* partial) {
+    const int64_t b = blockIdx.y;
+    const uint32_t per = (uint32_t)((cols + NORM_SPAN - 1) / NORM_SPAN);
+    const int64_t spans = rows * per;
     double s = 0;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)NORM_BLOCKS * 256) {
-        const float u = moved(io, b, i / io.cols, i % io.cols, true);
-        s += (double)u * (double)u;
+    for (int64_t i = blockIdx.x; i < spans; i += gridDim.x) {
+        const int64_t r = spans >> 31 ? i / per : (uint32_t)i / per, c0 = (i - r * per) * NORM_SPAN;
+        if (vec) {
+            const int64_t c = c0 + threadIdx.x * 8;
+            if (c < cols) {                                   // cols is a multiple of 8
+                T g[8];
+                float m[8];
+                const T* gp = io.grad + b * io.g_b + r * io.g_r + c;
+#pragma unroll
+                for (int v = 0; v < 8; v += 16 / (int)sizeof(T)) *(f32x4*)(g + v) = *(const f32x4*)(gp + v);
+                float* mp = io.mom + b * io.m_b + r * io.m_r + c;
+                if (io.mom) {
+                    *(f32x4*)m = *(const f32x4*)mp; *(f32x4*)(m + 4) = *(const f32x4*)(mp + 4);
+#pragma unroll
+                    for (int v = 0; v < 8; ++v) m[v] = io.beta * m[v] + (float)g[v];
+                    *(f32x4*)mp = *(f32x4*)m; *(f32x4*)(mp + 4) = *(f32x4*)(m + 4);
+                }
+#pragma unroll
+                for (int v = 0; v < 8; ++v) { const float u = !io.mom ? (float)g[v] : io.nesterov ? (float)g[v] + io.beta * m[v] : m[v]; s += (double)u * (double)u; }
+            }
+        } else {
+            for (int64_t c = c0 + threadIdx.x; c < cols && c < c0 + NORM_SPAN; c += 256) { const float u = moved(io, b, r, c, true); s += (double)u * (double)u; }
+        }
     }
     s = block_sum(s);
-    if (threadIdx.x == 0) partial[b * NORM_BLOCKS + blockIdx.x] = s;
+    if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = s;
 }
 
 template <bool SPLIT> __device__ inline void terms(float v, f16& hi, f16& lo) { hi = (f16)v; if constexpr (SPLIT) lo = (f16)(v - (float)hi); }
@@ -81,7 +108,8 @@ template <bool SPLIT> __device__ inline void terms(float v, f16& hi, f16& lo) { 
 template <class T, bool SPLIT> __global__ void __launch_bounds__(256) k_start(const Io<T> io, const Mat q) {
     __shared__ float tile[64][65];
     const int64_t b = blockIdx.z, i0 = (int64_t)blockIdx.y * 64, j0 = (int64_t)blockIdx.x * 64;      // rows and columns of X
-    double s = threadIdx.x < NORM_BLOCKS ? q.partial[b * NORM_BLOCKS + threadIdx.x] : 0.0;
+    double s = 0;
+    for (int i = threadIdx.x; i < q.nblocks; i += 256) s += q.partial[b * q.nblocks + i];
     s = block_sum(s);
     const double inv = (double)SX / (sqrt(s) + 1e-7);
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -109,8 +137,14 @@ template <class T, bool SPLIT> __global__ void __launch_bounds__(256) k_start(co
 
 // ---- products ---------------------------------------------------------------------------------------------------------------------------------------------------------
 // C[i][j] = sum_k P[i][k] Q[j][k] over padded sizes: both factors have k next to k.  A workgroup of four waves (2 x 2) takes a BT x BT tile, a wave BT / 2 x BT / 2 of it in
-// accumulators; stages of BK go through two LDS buffers, the next one in registers while this one is multiplied.  Chunk c of row r is stored at c ^ (r & 7): the eight
-// rows that a read touches together lie in different banks.
+// accumulators.  Stages of BK go from memory straight into one of four LDS buffers (no registers on the way), three stages ahead of the one that is multiplied.  Four distinct arrays, and
+// the stage loop unrolled by four: the compiler then knows that a read of one buffer need not wait for the requests that fill another.
+//
+// A request of a wave fills 1 KB of LDS in lane order: 16 rows of 64 bytes, four 16-byte chunks each.  Chunk c of row r lies at c ^ (r / 2 & 3): the lanes FETCH in that order, and the
+// eight rows that a read touches together then lie in different banks.
+//
+// In a stage the factors of its second half are read while the first half is multiplied, and those of the next stage's first half while the second is; the one barrier stands between the
+// halves: behind it the next stage has arrived in every wave's part, and no wave still reads this stage's buffer, which the stage after next but two is requested into.
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 
 struct Product {
@@ -124,11 +158,23 @@ struct Product {
 
 __device__ inline f32x16 mfma(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
+// Four neighbouring lanes hold four 16-bit values each, lane q those of column q; afterwards lane q holds row q.  Two exchanges of halves, with the lane two and then one apart.
+__device__ inline uint64_t across(uint64_t v, int quad) {
+    const uint32_t a = (uint32_t)v, b = (uint32_t)(v >> 32);                        // rows 0 1, rows 2 3
+    const uint32_t give = quad < 2 ? b : a, keep = quad < 2 ? a : b;
+    const uint32_t got = (uint32_t)__builtin_amdgcn_mov_dpp((int)give, 0x4e, 0xf, 0xf, true);      // quad_perm 2 3 0 1
+    const uint32_t c0 = quad < 2 ? keep : got, c1 = quad < 2 ? got : keep;          // this lane's two rows: columns (quad & 1), (quad & 1) + 2
+    const uint32_t d0 = (uint32_t)__builtin_amdgcn_mov_dpp((int)c0, 0xb1, 0xf, 0xf, true), d1 = (uint32_t)__builtin_amdgcn_mov_dpp((int)c1, 0xb1, 0xf, 0xf, true);
+    const uint32_t lo0 = quad & 1 ? (d0 >> 16) | (c0 & 0xffff0000u) : (c0 & 0xffffu) | (d0 << 16);
+    const uint32_t lo1 = quad & 1 ? (d1 >> 16) | (c1 & 0xffff0000u) : (c1 & 0xffffu) | (d1 << 16);
+    return (uint64_t)lo1 << 32 | lo0;
+}
+
 template <class T, int BT, int EPI, bool SPLIT>
 __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Product g, const Mat q, const Io<T> io, const int from, const int to) {
-    constexpr int CH = BT * 8 / 256;          // 16-byte chunks a thread moves per factor and stage
     constexpr int W = BT / 64;                // 32 x 32 accumulators a wave and direction
-    __shared__ __align__(16) f16 lds[2][2][BT * BK];
+    constexpr int RQ = BT / 64;               // requests of a wave, factor and stage
+    __shared__ __align__(16) f16 s0[2 * BT * BK], s1[2 * BT * BK], s2[2 * BT * BK], s3[2 * BT * BK];
     const int64_t b = blockIdx.z;
     int bi, bj;
     if constexpr (EPI == GRAM || EPI == POLY) {               // tile t of the lower triangle
@@ -147,119 +193,173 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
         for (int y = 0; y < W; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-    f16x8 gp[CH], gq[CH];
-    const int per = (int)(g.K / BK), stages = SPLIT ? 3 * per : per;
-    auto fetch = [&](int s) {
+    const int per = (int)(g.K / BK), stages = SPLIT ? 3 * per : per;              // multiples of four
+    const int64_t lane_at = (int64_t)(wave * RQ * 16 + (lane >> 2)) * g.K + (((lane & 3) ^ ((lane >> 3) & 3)) * 8), step_at = 16 * g.K;
+    auto request = [&](int s, f16* buf) {
+        s = s < stages ? s : stages - 1;                      // behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
         const int part = SPLIT ? s / per : 0, k = (SPLIT ? s % per : s) * BK;
-        const f16* P = g.P[SPLIT && part == 2 ? 1 : 0] + b * g.sP;
-        const f16* Q = g.Q[SPLIT && part == 1 ? 1 : 0] + b * g.sQ;
+        const f16* P = g.P[SPLIT && part == 2 ? 1 : 0] + b * g.sP + i0 * g.K + k + lane_at;
+        const f16* Q = g.Q[SPLIT && part == 1 ? 1 : 0] + b * g.sQ + j0 * g.K + k + lane_at;
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int id = c * 256 + tid, row = id >> 3, ch = id & 7;
-            gp[c] = *(const f16x8*)(P + (i0 + row) * g.K + k + ch * 8);
-            gq[c] = *(const f16x8*)(Q + (j0 + row) * g.K + k + ch * 8);
+        for (int c = 0; c < RQ; ++c) {
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(P + c * step_at), (__attribute__((address_space(3))) void*)(buf + (wave * RQ + c) * 512), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(Q + c * step_at), (__attribute__((address_space(3))) void*)(buf + BT * BK + (wave * RQ + c) * 512), 16, 0, 0);
         }
     };
-    auto stash = [&](int buf) {
+    const int rp = (wi * (BT / 2) + (lane & 31)) * BK, rq = BT * BK + (wj * (BT / 2) + (lane & 31)) * BK;
+    const int ch0 = ((lane >> 5) ^ ((lane >> 1) & 3)) * 8, ch1 = ((2 + (lane >> 5)) ^ ((lane >> 1) & 3)) * 8;
+    f16x8 p0[W], q0[W], p1[W], q1[W];
+    auto read = [&](const f16* buf, int ch, f16x8 (&fp)[W], f16x8 (&fq)[W]) {
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
-            const int id = c * 256 + tid, row = id >> 3, ch = (id & 7) ^ (row & 7);
-            *(f16x8*)&lds[buf][0][row * BK + ch * 8] = gp[c];
-            *(f16x8*)&lds[buf][1][row * BK + ch * 8] = gq[c];
-        }
+        for (int x = 0; x < W; ++x) { fp[x] = *(const f16x8*)(buf + rp + x * 32 * BK + ch); fq[x] = *(const f16x8*)(buf + rq + x * 32 * BK + ch); }
     };
-    fetch(0);
-    stash(0);
-    __syncthreads();
-    for (int s = 0; s < stages; ++s) {
-        if (s + 1 < stages) fetch(s + 1);
-        const f16* lp = lds[s & 1][0] + (wi * (BT / 2) + (lane & 31)) * BK;
-        const f16* lq = lds[s & 1][1] + (wj * (BT / 2) + (lane & 31)) * BK;
+    auto multiply = [&](const f16x8 (&fp)[W], const f16x8 (&fq)[W], int from, int to) {
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k) {
-            const int ch = ((k * 2 + (lane >> 5)) ^ (lane & 7)) * 8;          // (row & 7) == (lane & 7)
-            f16x8 fp[W], fq[W];
+        for (int x = from; x < to; ++x)
 #pragma unroll
-            for (int x = 0; x < W; ++x) { fp[x] = *(const f16x8*)(lp + x * 32 * BK + ch); fq[x] = *(const f16x8*)(lq + x * 32 * BK + ch); }
-#pragma unroll
-            for (int x = 0; x < W; ++x)
-#pragma unroll
-                for (int y = 0; y < W; ++y) acc[x][y] = mfma(fp[x], fq[y], acc[x][y]);
-        }
-        if (s + 1 < stages) stash((s + 1) & 1);
-        __syncthreads();
+            for (int y = 0; y < W; ++y) acc[x][y] = mfma(fp[x], fq[y], acc[x][y]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // the oldest stage in flight has arrived in this wave's part (those of two later ones, 2 RQ requests each, may still be on the way) and its LDS reads are done; then in all waves
+    auto arrive = [&]() {
+        static_assert(4 * RQ == 16 || 4 * RQ == 8, "the counts below");
+        __builtin_amdgcn_s_waitcnt(4 * RQ == 16 ? 0x4070 : 0x0078);               // vmcnt(4 RQ) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // reads are issued behind the first products of the other half: the wait before those would otherwise include them
+    auto stage = [&](int s, f16* now, const f16* next) {
+        multiply(p0, q0, 0, 1);
+        read(now, ch1, p1, q1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(p0, q0, 1, W);
+        arrive();
+        multiply(p1, q1, 0, 1);
+        read(next, ch0, p0, q0);
+        request(s + 4, now);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(p1, q1, 1, W);
+    };
+    request(0, s0); request(1, s1); request(2, s2);
+    __builtin_amdgcn_sched_barrier(0);
+    arrive();
+    request(3, s3);
+    read(s0, ch0, p0, q0);
+    for (int s = 0; s < stages; s += 4) {
+        stage(s, s0, s1);
+        stage(s + 1, s1, s2);
+        stage(s + 2, s2, s3);
+        stage(s + 3, s3, s0);
     }
-    // a lane holds, of each 32 x 32, column lane & 31 and rows 8 g + 4 (lane >> 5) + 0..3 for g = 0..3
+    __builtin_amdgcn_s_waitcnt(0x0070);                       // nothing is on the way to LDS when the workgroup ends
+    // A lane holds, of each 32 x 32, column lane & 31 and rows 8 g + 4 (lane >> 5) + 0..3 for g = 0..3: four neighbours of the transposed order.  For the other order four lanes
+    // exchange theirs, so that both are stored eight bytes at a time.  What a row of accumulators needs from memory is requested before any of it is used.
+    const int64_t jw = j0 + wj * (BT / 2) + (lane & 31), iw = i0 + wi * (BT / 2) + (lane >> 5) * 4;
+    const int quad = lane & 3;
 #pragma unroll
-    for (int x = 0; x < W; ++x)
+    for (int x = 0; x < W; ++x) {
+        f32x4 old[W][4];
+        if constexpr (EPI == POLY) {
+            f16x4 ah[W][4], al[W][4];
 #pragma unroll
-        for (int y = 0; y < W; ++y) {
-            const int64_t j = j0 + wj * (BT / 2) + y * 32 + (lane & 31);
+            for (int y = 0; y < W; ++y)
 #pragma unroll
-            for (int gq4 = 0; gq4 < 4; ++gq4) {
-                const int64_t i = i0 + wi * (BT / 2) + x * 32 + gq4 * 8 + (lane >> 5) * 4;
-                float v[4];
+                for (int h = 0; h < 4; ++h) {
+                    const int64_t at = b * q.mp * q.mp + (jw + y * 32) * q.mp + iw + x * 32 + h * 8;
+                    ah[y][h] = *(const f16x4*)(q.a[0] + at);
+                    if constexpr (SPLIT) al[y][h] = *(const f16x4*)(q.a[1] + at);
+                }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = acc[x][y][gq4 * 4 + r];
-                if constexpr (EPI == GRAM || EPI == POLY) {
-                    const int64_t at = b * q.mp * q.mp + j * q.mp + i;            // (j, i .. i + 3): the mirror image, four neighbours
-                    f16x4 hi, lo;
-                    if constexpr (EPI == GRAM) {
+            for (int y = 0; y < W; ++y)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] *= SA / (SX * SX);
+                for (int h = 0; h < 4; ++h)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) old[y][h][r] = SPLIT ? (float)ah[y][h][r] + (float)al[y][h][r] : (float)ah[y][h][r];
+        } else if constexpr (EPI == APPLY || EPI == LAST) {
+            if (!SPLIT && g.rounded) {
+                f16x4 xh[W][4];
+#pragma unroll
+                for (int y = 0; y < W; ++y)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) xh[y][h] = *(const f16x4*)(q.xt[from][0] + (b * q.np + jw + y * 32) * q.mp + iw + x * 32 + h * 8);
+#pragma unroll
+                for (int y = 0; y < W; ++y)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) old[y][h][r] = (float)xh[y][h][r];
+            } else {
+#pragma unroll
+                for (int y = 0; y < W; ++y)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) old[y][h] = *(const f32x4*)(q.master + (b * q.np + jw + y * 32) * q.mp + iw + x * 32 + h * 8);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int y = 0; y < W; ++y)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const int64_t i = iw + x * 32 + h * 8, j = jw + y * 32;            // rows i .. i + 3 of column j
+                f32x4 v;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    v[r] = acc[x][y][h * 4 + r];
+                    if constexpr (EPI == GRAM) v[r] *= SA / (SX * SX);
+                    else if constexpr (EPI == POLY) v[r] = g.c1 * old[y][h][r] + g.c2 * (v[r] * (1.f / SA));
+                    else v[r] = g.c0 * old[y][h][r] + v[r] * (1.f / SA);
+                }
+                if constexpr (EPI == LAST) {
+                    const float f = io.scale * (1.f / SX);
+                    T o[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[r] = (T)(v[r] * f);
+                    if (q.flip) {
+                        if (j < q.n) {
+                            T* dst = io.out + b * io.o_b + j * io.o_r + i;
+                            if (io.vec && i + 4 <= q.m) {
+                                if constexpr (sizeof(T) == 2) *(uint64_t*)dst = __builtin_bit_cast(uint64_t, *(f16x4*)o); else *(f32x4*)dst = *(f32x4*)o;
+                            } else {
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) if (i + r < q.m) dst[r] = o[r];
+                            }
+                        }
                     } else {
-                        const f16x4 ah = *(const f16x4*)(q.a[0] + at);
-                        f16x4 al = {};
-                        if constexpr (SPLIT) al = *(const f16x4*)(q.a[1] + at);
+                        if constexpr (sizeof(T) == 2) {
+                            const uint64_t row = across(__builtin_bit_cast(uint64_t, *(f16x4*)o), quad);
+                            const int64_t jq = j - quad;
+                            if (i + quad < q.m) {
+                                T* dst = io.out + b * io.o_b + (i + quad) * io.o_r + jq;
+                                if (io.vec && jq + 4 <= q.n) *(uint64_t*)dst = row;
+                                else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = g.c1 * ((float)ah[r] + (float)al[r]) + g.c2 * (v[r] * (1.f / SA));
-                    }
-                    f16* const* dst = EPI == GRAM ? q.a : q.b;
+                                    for (int r = 0; r < 4; ++r) if (jq + r < q.n) ((uint16_t*)dst)[r] = (uint16_t)(row >> (16 * r));
+                                }
+                            }
+                        } else if (j < q.n) {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) { f16 h, l = 0; terms<SPLIT>(v[r], h, l); hi[r] = h; lo[r] = l; }
-                    *(f16x4*)(dst[0] + at) = hi;
-                    if constexpr (SPLIT) *(f16x4*)(dst[1] + at) = lo;
-                    if (bi != bj) {
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int64_t d = b * q.mp * q.mp + (i + r) * q.mp + j;
-                            dst[0][d] = hi[r];
-                            if constexpr (SPLIT) dst[1][d] = lo[r];
+                            for (int r = 0; r < 4; ++r) if (i + r < q.m) io.out[b * io.o_b + (i + r) * io.o_r + j] = o[r];
                         }
                     }
                 } else {
-                    const int64_t att = (b * q.np + j) * q.mp + i;
-                    f32x4 old;
-                    if (g.rounded) {
-                        const f16x4 xh = *(const f16x4*)(q.xt[from][0] + att);
+                    f16x4 hi, lo;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) old[r] = (float)xh[r];
-                    } else old = *(const f32x4*)(q.master + att);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) v[r] = g.c0 * old[r] + v[r] * (1.f / SA);
-                    if constexpr (EPI == APPLY) {
-                        f16x4 hi, lo;
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) { f16 h, l = 0; terms<SPLIT>(v[r], h, l); hi[r] = h; lo[r] = l; }
-                        *(f16x4*)(q.xt[to][0] + att) = hi;
-                        if constexpr (SPLIT) *(f16x4*)(q.xt[to][1] + att) = lo;
-                        if (g.keep) { f32x4 o; for (int r = 0; r < 4; ++r) o[r] = v[r]; *(f32x4*)(q.master + att) = o; }
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const int64_t d = (b * q.mp + i + r) * q.np + j;
-                            q.x[0][d] = hi[r];
-                            if constexpr (SPLIT) q.x[1][d] = lo[r];
-                        }
-                    } else {
-                        if (j < q.n) {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (i + r < q.m) io.out[b * io.o_b + (q.flip ? j * io.o_r + i + r : (i + r) * io.o_r + j)] = (T)(v[r] * (io.scale * (1.f / SX)));
-                        }
+                    for (int r = 0; r < 4; ++r) { f16 e, l = 0; terms<SPLIT>(v[r], e, l); hi[r] = e; lo[r] = l; }
+                    constexpr bool SQUARE = EPI == GRAM || EPI == POLY;
+                    f16* const* direct = EPI == GRAM ? q.a : EPI == POLY ? q.b : q.x;
+                    f16* const* turned = EPI == GRAM ? q.a : EPI == POLY ? q.b : q.xt[to];
+                    const int64_t att = SQUARE ? (b * q.mp + j) * q.mp + i : (b * q.np + j) * q.mp + i;
+                    const int64_t atd = SQUARE ? (b * q.mp + i + quad) * q.mp + j - quad : (b * q.mp + i + quad) * q.np + j - quad;
+                    *(f16x4*)(turned[0] + att) = hi;
+                    if constexpr (SPLIT) *(f16x4*)(turned[1] + att) = lo;
+                    if constexpr (EPI == APPLY) { if (g.keep) *(f32x4*)(q.master + att) = v; }
+                    if (!SQUARE || bi != bj) {
+                        *(uint64_t*)(direct[0] + atd) = across(__builtin_bit_cast(uint64_t, hi), quad);
+                        if constexpr (SPLIT) *(uint64_t*)(direct[1] + atd) = across(__builtin_bit_cast(uint64_t, lo), quad);
                     }
                 }
             }
-        }
+    }
 }
 
 }  // namespace orth

@@ -34,7 +34,8 @@ static Plan plan_of(const hipadj_orthogonal* o, char* base) {
         q.b[t] = (f16*)take(q.batch * q.mp * q.mp * 2);
     }
     q.master = (float*)take(q.batch * q.mp * q.np * 4);
-    q.partial = (double*)take(q.batch * NORM_BLOCKS * 8);
+    q.nblocks = (int)std::max<int64_t>(1, std::min<int64_t>({NORM_BLOCKS, (q.m * q.n + NORM_SPAN - 1) / NORM_SPAN, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, q.batch))}));
+    q.partial = (double*)take(q.batch * q.nblocks * 8);
     p.bytes = at;
     return p;
 }
@@ -45,8 +46,17 @@ template <class T, int BT, int EPI, bool SPLIT> static void product(const Produc
     k_product<T, BT, EPI, SPLIT><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
 }
 
+template <class T, int EPI, bool SPLIT> static void product_of(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
+    if ((EPI == APPLY || EPI == LAST) && g.M % 256 == 0 && g.N % 256 == 0 && g.M / 256 * (g.N / 256) * q.batch >= 192) product<T, 256, EPI, SPLIT>(g, q, io, from, to, s);
+    else product<T, 128, EPI, SPLIT>(g, q, io, from, to, s);
+}
+
 template <class T, int BT, bool SPLIT> static void iterate(const hipadj_orthogonal* o, const Mat& q, const Io<T>& io, hipStream_t s) {
-    k_norm<T><<<dim3(NORM_BLOCKS, (uint32_t)q.batch), dim3(256), 0, s>>>(io, q.partial);
+    const bool flat = io.g_r == io.cols && (!io.mom || io.m_r == io.cols);
+    const int64_t rows = flat ? 1 : io.rows, cols = flat ? io.rows * io.cols : io.cols;
+    auto aligned = [&](const void* p, int64_t sb, int64_t sr, int64_t per) { return (uintptr_t)p % 16 == 0 && (q.batch == 1 || sb % per == 0) && (rows == 1 || sr % per == 0); };
+    const bool vec = cols % 8 == 0 && aligned(io.grad, io.g_b, io.g_r, 16 / sizeof(T)) && (!io.mom || aligned(io.mom, io.m_b, io.m_r, 4));
+    k_norm<T><<<dim3((uint32_t)q.nblocks, (uint32_t)q.batch), dim3(256), 0, s>>>(io, rows, cols, vec, q.partial);
     k_start<T, SPLIT><<<dim3((uint32_t)(q.np / 64), (uint32_t)(q.mp / 64), (uint32_t)q.batch), dim3(256), 0, s>>>(io, q);
     const int64_t smm = q.mp * q.mp, smn = q.mp * q.np;
     auto rounded = [&](int step) { return !SPLIT && step >= o->steps - 2; };
@@ -56,14 +66,14 @@ template <class T, int BT, bool SPLIT> static void iterate(const hipadj_orthogon
         Product g{};
         g.c0 = (float)c[0]; g.c1 = (float)c[1]; g.c2 = (float)c[2];
         g.P[0] = g.Q[0] = q.x[0]; g.P[1] = g.Q[1] = q.x[1]; g.sP = g.sQ = smn; g.K = q.np; g.M = g.N = q.mp;
-        product<T, BT, GRAM, SPLIT>(g, q, io, from, to, s);
+        product_of<T, GRAM, SPLIT>(g, q, io, from, to, s);
         g.P[0] = g.Q[0] = q.a[0]; g.P[1] = g.Q[1] = q.a[1]; g.sP = g.sQ = smm; g.K = q.mp;
-        product<T, BT, POLY, SPLIT>(g, q, io, from, to, s);
+        product_of<T, POLY, SPLIT>(g, q, io, from, to, s);
         g.P[0] = q.b[0]; g.P[1] = q.b[1]; g.sP = smm;
         g.Q[0] = q.xt[from][0]; g.Q[1] = q.xt[from][1]; g.sQ = smn; g.N = q.np;
         g.rounded = rounded(step); g.keep = !rounded(step + 1);
-        if (step + 1 < o->steps) product<T, BT, APPLY, SPLIT>(g, q, io, from, to, s);
-        else product<T, BT, LAST, SPLIT>(g, q, io, from, to, s);
+        if (step + 1 < o->steps) product_of<T, APPLY, SPLIT>(g, q, io, from, to, s);
+        else product_of<T, LAST, SPLIT>(g, q, io, from, to, s);
     }
 }
 
@@ -72,6 +82,7 @@ template <class T> static void run(const hipadj_orthogonal* o, const Plan& p, co
     io.grad = (const T*)grad; io.mom = mom; io.out = (T*)out; io.rows = o->rows; io.cols = o->cols;
     io.g_b = o->grad_stride[0]; io.g_r = o->grad_stride[1]; io.m_b = o->momentum_stride[0]; io.m_r = o->momentum_stride[1]; io.o_b = o->out_stride[0]; io.o_r = o->out_stride[1];
     io.beta = (float)o->beta; io.scale = (float)o->scale; io.nesterov = o->nesterov;
+    io.vec = (uintptr_t)out % (4 * sizeof(T)) == 0 && io.o_r % 4 == 0 && (o->batch == 1 || io.o_b % 4 == 0);
     if (p.split) iterate<T, 128, true>(o, p.q, io, s);
     else if constexpr (sizeof(T) == 2) iterate<T, 128, false>(o, p.q, io, s);
 }
