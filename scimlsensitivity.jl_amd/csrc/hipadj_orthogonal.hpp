@@ -140,11 +140,11 @@ template <class T, bool SPLIT> __global__ void __launch_bounds__(256) k_start(co
 // accumulators.  Stages of BK go from memory straight into one of four LDS buffers (no registers on the way), three stages ahead of the one that is multiplied.  Four distinct arrays, and
 // the stage loop unrolled by four: the compiler then knows that a read of one buffer need not wait for the requests that fill another.
 //
-// A request of a wave fills 1 KB of LDS in lane order: 16 rows of 64 bytes, four 16-byte chunks each.  Chunk c of row r lies at c ^ (r / 2 & 3): the lanes FETCH in that order, and the
-// eight rows that a read touches together then lie in different banks.
+// A request of a wave fills 1 KB of LDS in lane order: 16 rows of 64 bytes, four 16-byte chunks each.  Chunk c of row r lies at c ^ (r / 4 & 3): the lanes FETCH in that order, and the
+// sixteen rows that a read touches together then lie in different ones of the 64 banks (with r / 2 & 3 half of the LDS cycles were conflicts).
 //
 // In a stage the factors of its second half are read while the first half is multiplied, and those of the next stage's first half while the second is; the one barrier stands between the
-// halves: behind it the next stage has arrived in every wave's part, and no wave still reads this stage's buffer, which the stage after next but two is requested into.
+// halves: behind it the next stage has arrived in every wave's part, and no wave still reads this stage's buffer, which stage s + 4 is requested into.
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 
 struct Product {
@@ -183,7 +183,14 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
         while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
         while (bi * (bi + 1) / 2 > t) --bi;
         bj = t - bi * (bi + 1) / 2;
-    } else { bi = blockIdx.y; bj = blockIdx.x; }
+    } else {
+        // workgroups go round the eight XCDs: each gets a compact part of the tiles (2 x 4 parts), so that its L2 serves its factors' rows to all of them
+        const int ti = (int)((g.M + BT - 1) / BT), tj = (int)((g.N + BT - 1) / BT), t = blockIdx.x;
+        if (ti % 2 == 0 && tj % 4 == 0) {
+            const int x = t & 7, u = t >> 3, wj4 = tj / 4;
+            bi = (x >> 2) * (ti / 2) + u / wj4; bj = (x & 3) * wj4 + u % wj4;
+        } else { bi = t / tj; bj = t % tj; }
+    }
     const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, wi = wave >> 1, wj = wave & 1;
     const int64_t i0 = (int64_t)bi * BT, j0 = (int64_t)bj * BT;
     f32x16 acc[W][W];
@@ -194,70 +201,84 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
     const int per = (int)(g.K / BK), stages = SPLIT ? 3 * per : per;              // multiples of four
-    const int64_t lane_at = (int64_t)(wave * RQ * 16 + (lane >> 2)) * g.K + (((lane & 3) ^ ((lane >> 3) & 3)) * 8), step_at = 16 * g.K;
-    auto request = [&](int s, f16* buf) {
-        s = s < stages ? s : stages - 1;                      // behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
-        const int part = SPLIT ? s / per : 0, k = (SPLIT ? s % per : s) * BK;
-        const f16* P = g.P[SPLIT && part == 2 ? 1 : 0] + b * g.sP + i0 * g.K + k + lane_at;
-        const f16* Q = g.Q[SPLIT && part == 1 ? 1 : 0] + b * g.sQ + j0 * g.K + k + lane_at;
+    // rows past the last one (the sides are multiples of 128, not of every BT) are requested from the last one, multiplied and not stored
+    int64_t row_p[RQ], row_q[RQ];
 #pragma unroll
-        for (int c = 0; c < RQ; ++c) {
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(P + c * step_at), (__attribute__((address_space(3))) void*)(buf + (wave * RQ + c) * 512), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(Q + c * step_at), (__attribute__((address_space(3))) void*)(buf + BT * BK + (wave * RQ + c) * 512), 16, 0, 0);
-        }
+    for (int c = 0; c < RQ; ++c) {
+        const int64_t r = (wave * RQ + c) * 16 + (lane >> 2), k = ((lane & 3) ^ ((lane >> 4) & 3)) * 8;
+        row_p[c] = (i0 + r < g.M ? i0 + r : g.M - 1) * g.K + k;
+        row_q[c] = (j0 + r < g.N ? j0 + r : g.N - 1) * g.K + k;
+    }
+    // requests n of the 2 RQ of a stage; behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
+    auto request = [&](int s, f16* buf, int n) {
+        s = s < stages ? s : stages - 1;
+        const int part = SPLIT ? s / per : 0, k = (SPLIT ? s % per : s) * BK, c = n % RQ;
+        const f16* from = n < RQ ? g.P[SPLIT && part == 2 ? 1 : 0] + b * g.sP + k + row_p[c] : g.Q[SPLIT && part == 1 ? 1 : 0] + b * g.sQ + k + row_q[c];
+        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                         (__attribute__((address_space(3))) void*)(buf + (n < RQ ? 0 : BT * BK) + (wave * RQ + c) * 512), 16, 0, 0);
     };
     const int rp = (wi * (BT / 2) + (lane & 31)) * BK, rq = BT * BK + (wj * (BT / 2) + (lane & 31)) * BK;
-    const int ch0 = ((lane >> 5) ^ ((lane >> 1) & 3)) * 8, ch1 = ((2 + (lane >> 5)) ^ ((lane >> 1) & 3)) * 8;
+    const int ch0 = ((lane >> 5) ^ ((lane >> 2) & 3)) * 8, ch1 = ((2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 8;
     f16x8 p0[W], q0[W], p1[W], q1[W];
-    auto read = [&](const f16* buf, int ch, f16x8 (&fp)[W], f16x8 (&fq)[W]) {
-#pragma unroll
-        for (int x = 0; x < W; ++x) { fp[x] = *(const f16x8*)(buf + rp + x * 32 * BK + ch); fq[x] = *(const f16x8*)(buf + rq + x * 32 * BK + ch); }
+    auto read = [&](const f16* buf, int ch, f16x8 (&fp)[W], f16x8 (&fq)[W], int n) {      // n of the 2 W factors
+        if (n < W) fp[n] = *(const f16x8*)(buf + rp + n * 32 * BK + ch);
+        else fq[n - W] = *(const f16x8*)(buf + rq + (n - W) * 32 * BK + ch);
     };
-    auto multiply = [&](const f16x8 (&fp)[W], const f16x8 (&fq)[W], int from, int to) {
+    // half a stage: the products of one half with the reads of the next and RQ requests between them, one at a time — issued in a burst they hold the wave, and with it the matrix
+    // core, up to the rate of the request queue and of LDS
+    auto half = [&](const f16x8 (&fp)[W], const f16x8 (&fq)[W], const f16* rbuf, int ch, f16x8 (&np)[W], f16x8 (&nq)[W], int rs, f16* qbuf, int n0) {
+        int reads = 0, requests = 0;
 #pragma unroll
-        for (int x = from; x < to; ++x)
+        for (int m = 0; m < W * W; ++m) {
+            const int x = m / W, y = m % W;
+            acc[x][y] = mfma(fp[x], fq[y], acc[x][y]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int y = 0; y < W; ++y) acc[x][y] = mfma(fp[x], fq[y], acc[x][y]);
-        __builtin_amdgcn_sched_barrier(0);
+            for (; reads < 2 * W && reads * W <= (m + 1) * 3 - 1; ++reads) read(rbuf, ch, np, nq, reads);     // all within the first two thirds
+            if (requests < RQ && (m + 1) * RQ >= (requests + 1) * W * W) { request(rs, qbuf, n0 + requests); ++requests; }
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
     // the oldest stage in flight has arrived in this wave's part (those of two later ones, 2 RQ requests each, may still be on the way) and its LDS reads are done; then in all waves
     auto arrive = [&]() {
-        static_assert(4 * RQ == 16 || 4 * RQ == 8, "the counts below");
-        __builtin_amdgcn_s_waitcnt(4 * RQ == 16 ? 0x4070 : 0x0078);               // vmcnt(4 RQ) lgkmcnt(0)
+        static_assert(RQ >= 2 && RQ <= 4, "the counts below");
+        __builtin_amdgcn_s_waitcnt(RQ == 4 ? 0x4070 : RQ == 3 ? 0x007c : 0x0078);  // vmcnt(4 RQ) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
-    // reads are issued behind the first products of the other half: the wait before those would otherwise include them
-    auto stage = [&](int s, f16* now, const f16* next) {
-        multiply(p0, q0, 0, 1);
-        read(now, ch1, p1, q1);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(p0, q0, 1, W);
+    // behind the barrier no wave reads `now` any more: its next stage is requested half there, half in the first half of the next stage
+    auto stage = [&](int s, f16* prev, f16* now, const f16* next) {
+        half(p0, q0, now, ch1, p1, q1, s + 3, prev, RQ);
         arrive();
-        multiply(p1, q1, 0, 1);
-        read(next, ch0, p0, q0);
-        request(s + 4, now);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(p1, q1, 1, W);
+        half(p1, q1, next, ch0, p0, q0, s + 4, now, 0);
     };
-    request(0, s0); request(1, s1); request(2, s2);
+    auto all = [&](int s, f16* buf, int from, int to) {
+#pragma unroll
+        for (int n = from; n < to; ++n) request(s, buf, n);
+    };
+    all(0, s0, 0, 2 * RQ); all(1, s1, 0, 2 * RQ); all(2, s2, 0, 2 * RQ);
     __builtin_amdgcn_sched_barrier(0);
     arrive();
-    request(3, s3);
-    read(s0, ch0, p0, q0);
+    all(3, s3, 0, RQ);
+#pragma unroll
+    for (int n = 0; n < 2 * W; ++n) read(s0, ch0, p0, q0, n);
     for (int s = 0; s < stages; s += 4) {
-        stage(s, s0, s1);
-        stage(s + 1, s1, s2);
-        stage(s + 2, s2, s3);
-        stage(s + 3, s3, s0);
+        stage(s, s3, s0, s1);
+        stage(s + 1, s0, s1, s2);
+        stage(s + 2, s1, s2, s3);
+        stage(s + 3, s2, s3, s0);
     }
     __builtin_amdgcn_s_waitcnt(0x0070);                       // nothing is on the way to LDS when the workgroup ends
     // A lane holds, of each 32 x 32, column lane & 31 and rows 8 g + 4 (lane >> 5) + 0..3 for g = 0..3: four neighbours of the transposed order.  For the other order four lanes
     // exchange theirs, so that both are stored eight bytes at a time.  What a row of accumulators needs from memory is requested before any of it is used.
     const int64_t jw = j0 + wj * (BT / 2) + (lane & 31), iw = i0 + wi * (BT / 2) + (lane >> 5) * 4;
     const int quad = lane & 3;
+    int64_t jc[W];                                            // columns that are read: inside
+#pragma unroll
+    for (int y = 0; y < W; ++y) jc[y] = jw + y * 32 < g.N ? jw + y * 32 : jw < g.N ? jw : 0;
 #pragma unroll
     for (int x = 0; x < W; ++x) {
+        if (i0 + wi * (BT / 2) + x * 32 >= g.M) continue;     // the same for all lanes
         f32x4 old[W][4];
         if constexpr (EPI == POLY) {
             f16x4 ah[W][4], al[W][4];
@@ -265,7 +286,7 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
             for (int y = 0; y < W; ++y)
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    const int64_t at = b * q.mp * q.mp + (jw + y * 32) * q.mp + iw + x * 32 + h * 8;
+                    const int64_t at = b * q.mp * q.mp + jc[y] * q.mp + iw + x * 32 + h * 8;
                     ah[y][h] = *(const f16x4*)(q.a[0] + at);
                     if constexpr (SPLIT) al[y][h] = *(const f16x4*)(q.a[1] + at);
                 }
@@ -281,7 +302,7 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
 #pragma unroll
                 for (int y = 0; y < W; ++y)
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) xh[y][h] = *(const f16x4*)(q.xt[from][0] + (b * q.np + jw + y * 32) * q.mp + iw + x * 32 + h * 8);
+                    for (int h = 0; h < 4; ++h) xh[y][h] = *(const f16x4*)(q.xt[from][0] + (b * q.np + jc[y]) * q.mp + iw + x * 32 + h * 8);
 #pragma unroll
                 for (int y = 0; y < W; ++y)
 #pragma unroll
@@ -292,12 +313,13 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
 #pragma unroll
                 for (int y = 0; y < W; ++y)
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) old[y][h] = *(const f32x4*)(q.master + (b * q.np + jw + y * 32) * q.mp + iw + x * 32 + h * 8);
+                    for (int h = 0; h < 4; ++h) old[y][h] = *(const f32x4*)(q.master + (b * q.np + jc[y]) * q.mp + iw + x * 32 + h * 8);
             }
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int y = 0; y < W; ++y)
+        for (int y = 0; y < W; ++y) {
+            if (j0 + wj * (BT / 2) + y * 32 >= g.N) continue;
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
                 const int64_t i = iw + x * 32 + h * 8, j = jw + y * 32;            // rows i .. i + 3 of column j
@@ -359,6 +381,7 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
                     }
                 }
             }
+        }
     }
 }
 

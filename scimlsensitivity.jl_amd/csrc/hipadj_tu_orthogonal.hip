@@ -40,18 +40,31 @@ static Plan plan_of(const hipadj_orthogonal* o, char* base) {
     return p;
 }
 
+static int64_t tiles_of(const Product& g, int64_t batch, bool lower, int64_t BT) {
+    const int64_t ti = (g.M + BT - 1) / BT, tj = (g.N + BT - 1) / BT;
+    return (lower ? ti * (ti + 1) / 2 : ti * tj) * batch;
+}
 template <class T, int BT, int EPI, bool SPLIT> static void product(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
-    const int64_t ti = g.M / BT, tj = g.N / BT;
-    const dim3 grid = EPI == GRAM || EPI == POLY ? dim3((uint32_t)(ti * (ti + 1) / 2), 1, (uint32_t)q.batch) : dim3((uint32_t)tj, (uint32_t)ti, (uint32_t)q.batch);
+    const dim3 grid((uint32_t)tiles_of(g, 1, EPI == GRAM || EPI == POLY, BT), 1, (uint32_t)q.batch);
     k_product<T, BT, EPI, SPLIT><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
 }
 
+// The tile of a product: the one whose rounds over the 256 CUs take the least.  Measured, nanoseconds a row of K: a 256 tile 31, a 192 tile 19, a 128 tile 9.5, two of which share a CU (20).
+// Larger tiles read less LDS a product, smaller ones leave fewer CUs without work: 4096 x 4096 by symmetric halves is 253 tiles of 192 (one round), 136 of 256, 528 of 128.
 template <class T, int EPI, bool SPLIT> static void product_of(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
-    if ((EPI == APPLY || EPI == LAST) && g.M % 256 == 0 && g.N % 256 == 0 && g.M / 256 * (g.N / 256) * q.batch >= 192) product<T, 256, EPI, SPLIT>(g, q, io, from, to, s);
+    auto cost = [&](int64_t BT) -> double {
+        const int64_t n = tiles_of(g, q.batch, EPI == GRAM || EPI == POLY, BT);
+        if (BT != 128) return (double)((n + 255) / 256) * (BT == 256 ? 31.0 : 19.0);
+        const int64_t left = n % 512;
+        return (double)(n / 512) * 20.0 + (left > 256 ? 20.0 : left ? 9.5 : 0.0);
+    };
+    const double c128 = cost(128), c192 = cost(192), c256 = cost(256);
+    if (c256 <= c192 && c256 <= c128) product<T, 256, EPI, SPLIT>(g, q, io, from, to, s);
+    else if (c192 <= c128) product<T, 192, EPI, SPLIT>(g, q, io, from, to, s);
     else product<T, 128, EPI, SPLIT>(g, q, io, from, to, s);
 }
 
-template <class T, int BT, bool SPLIT> static void iterate(const hipadj_orthogonal* o, const Mat& q, const Io<T>& io, hipStream_t s) {
+template <class T, bool SPLIT> static void iterate(const hipadj_orthogonal* o, const Mat& q, const Io<T>& io, hipStream_t s) {
     const bool flat = io.g_r == io.cols && (!io.mom || io.m_r == io.cols);
     const int64_t rows = flat ? 1 : io.rows, cols = flat ? io.rows * io.cols : io.cols;
     auto aligned = [&](const void* p, int64_t sb, int64_t sr, int64_t per) { return (uintptr_t)p % 16 == 0 && (q.batch == 1 || sb % per == 0) && (rows == 1 || sr % per == 0); };
@@ -83,8 +96,8 @@ template <class T> static void run(const hipadj_orthogonal* o, const Plan& p, co
     io.g_b = o->grad_stride[0]; io.g_r = o->grad_stride[1]; io.m_b = o->momentum_stride[0]; io.m_r = o->momentum_stride[1]; io.o_b = o->out_stride[0]; io.o_r = o->out_stride[1];
     io.beta = (float)o->beta; io.scale = (float)o->scale; io.nesterov = o->nesterov;
     io.vec = (uintptr_t)out % (4 * sizeof(T)) == 0 && io.o_r % 4 == 0 && (o->batch == 1 || io.o_b % 4 == 0);
-    if (p.split) iterate<T, 128, true>(o, p.q, io, s);
-    else if constexpr (sizeof(T) == 2) iterate<T, 128, false>(o, p.q, io, s);
+    if (p.split) iterate<T, true>(o, p.q, io, s);
+    else if constexpr (sizeof(T) == 2) iterate<T, false>(o, p.q, io, s);
 }
 
 // How far the coefficients let the iteration grow: X starts with singular values in [0, 1], a step maps a bound s to the largest |c0 x + c1 x^3 + c2 x^5| on [0, s], reached at s or where
