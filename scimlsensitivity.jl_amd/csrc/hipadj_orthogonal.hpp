@@ -41,6 +41,9 @@ struct Mat {                                  // one batch of matrices and the w
 };
 constexpr int NORM_BLOCKS = 1024;             // at most; Mat::nblocks of them
 
+constexpr int MOST_STEPS = 64;
+struct Coefficients { float c[3 * MOST_STEPS]; };
+
 // ---- gradient, momentum, norm -------------------------------------------------------------------------------------------------------------------------------------------
 template <class T> struct Io {
     const T* grad; float* mom; T* out;
@@ -383,6 +386,108 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
             }
         }
     }
+}
+
+// ---- small matrices ---------------------------------------------------------------------------------------------------------------------------------------------------
+// Both sides at most 128: one workgroup does a matrix in one launch (17 otherwise, each a few microseconds of latency).  X, A and B live in LDS as two F16 terms and 32 x 32 pieces of X
+// stay in the F32 registers of the waves that own them.  X is needed by rows for X X' and by columns for B X, never at once, and A, B never next to X by rows: two regions, 128 KB at
+// a side of 128.  Symmetric matrices are stored transposed, which is their own order, four neighbours at a time.
+template <class T, int S> __global__ void __launch_bounds__((S / 32) * (S / 32) * 64) k_small(const Io<T> io, const int64_t m, const int64_t n, const bool flip, const int steps, const Coefficients co) {
+    constexpr int WS = S / 32, NWAVE = WS * WS, CHUNKS = S / 8;
+    __shared__ __align__(16) f16 x[2][S * S], a[2][S * S];
+    __shared__ double part[NWAVE];
+    const int64_t b = blockIdx.x;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, wi = wave / WS, wj = wave % WS, quad = lane & 3;
+    const int j = wj * 32 + (lane & 31), i0 = wi * 32 + (lane >> 5) * 4;            // this lane's elements: rows i0 + 8 h + r of column j
+    // place of the 16-byte chunk c of a row
+    auto at = [](int row, int c) { return row * S + ((c ^ (S == 128 ? row & 15 : S == 64 ? row >> 1 & 7 : row >> 2 & 3)) * 8); };
+    float v[4][4];
+    double sum = 0;
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = i0 + 8 * h + r;
+            v[h][r] = i < m && j < n ? (flip ? moved(io, b, j, i, true) : moved(io, b, i, j, true)) : 0.f;
+            sum += (double)v[h][r] * (double)v[h][r];
+        }
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) part[wave] = sum;
+    __syncthreads();
+    sum = 0;
+    for (int w = 0; w < NWAVE; ++w) sum += part[w];
+    const double inv = (double)SX / (sqrt(sum) + 1e-7);
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[h][r] = (float)((double)v[h][r] * inv);
+    auto split = [&](const float (&f)[4], uint64_t& hi, uint64_t& lo) {
+        f16x4 eh, el;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { f16 p, q; terms<true>(f[r], p, q); eh[r] = p; el[r] = q; }
+        hi = __builtin_bit_cast(uint64_t, eh); lo = __builtin_bit_cast(uint64_t, el);
+    };
+    auto put_columns = [&](f16 (&dst)[2][S * S], const float (&f)[4][4]) {          // (column j, rows i ..): by columns, or a symmetric matrix
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            uint64_t hi, lo;
+            split(f[h], hi, lo);
+            const int i = i0 + 8 * h, w = at(j, i >> 3) + (i & 7);
+            *(uint64_t*)&dst[0][w] = hi; *(uint64_t*)&dst[1][w] = lo;
+        }
+    };
+    auto put_rows = [&](f16 (&dst)[2][S * S], const float (&f)[4][4]) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            uint64_t hi, lo;
+            split(f[h], hi, lo);
+            const int i = i0 + 8 * h + quad, jq = j - quad, w = at(i, jq >> 3) + (jq & 7);
+            *(uint64_t*)&dst[0][w] = across(hi, quad); *(uint64_t*)&dst[1][w] = across(lo, quad);
+        }
+    };
+    auto product = [&](const f16 (&P)[2][S * S], const f16 (&Q)[2][S * S]) {        // rows 32 wi .. of P times rows 32 wj .. of Q
+        f32x16 acc;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+        const int rp = wi * 32 + (lane & 31), rq = wj * 32 + (lane & 31);
+#pragma unroll 2
+        for (int c = 0; c < CHUNKS; c += 2) {
+            const int k = c + (lane >> 5);
+            const f16x8 ph = *(const f16x8*)&P[0][at(rp, k)], pl = *(const f16x8*)&P[1][at(rp, k)], qh = *(const f16x8*)&Q[0][at(rq, k)], ql = *(const f16x8*)&Q[1][at(rq, k)];
+            acc = mfma(ph, ql, acc); acc = mfma(pl, qh, acc); acc = mfma(ph, qh, acc);
+        }
+        return acc;
+    };
+    put_rows(x, v);
+    for (int s = 0; s < steps; ++s) {
+        const float c0 = co.c[3 * s], c1 = co.c[3 * s + 1], c2 = co.c[3 * s + 2];
+        float g[4][4];
+        __syncthreads();
+        f32x16 acc = product(x, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) g[e >> 2][e & 3] = acc[e] * (SA / (SX * SX));
+        put_columns(a, g);
+        __syncthreads();
+        acc = product(a, a);
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) g[e >> 2][e & 3] = c1 * g[e >> 2][e & 3] + c2 * (acc[e] * (1.f / SA));
+        put_columns(a, g);
+        put_columns(x, v);
+        __syncthreads();
+        acc = product(a, x);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[e >> 2][e & 3] = c0 * v[e >> 2][e & 3] + acc[e] * (1.f / SA);
+        if (s + 1 < steps) { __syncthreads(); put_rows(x, v); }
+    }
+    const float f = io.scale * (1.f / SX);
+#pragma unroll
+    for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int i = i0 + 8 * h + r;
+            if (i < m && j < n) io.out[b * io.o_b + (flip ? (int64_t)j * io.o_r + i : (int64_t)i * io.o_r + j)] = (T)(v[h][r] * f);
+        }
 }
 
 }  // namespace orth

@@ -7,7 +7,7 @@
 
 namespace orth {
 
-struct Plan { Mat q; bool split; int64_t bytes; };
+struct Plan { Mat q; bool split, small; int64_t bytes; };
 
 static int64_t padded(int64_t v) { return (v + PADDED - 1) / PADDED * PADDED; }
 
@@ -22,6 +22,9 @@ static Plan plan_of(const hipadj_orthogonal* o, char* base) {
     q.mp = padded(q.m); q.np = padded(q.n);
     q.batch = o->batch;
     p.split = !one_term(o);
+    p.small = q.n <= 128;
+    p.bytes = 0;
+    if (p.small) return p;
     int64_t at = 0;
     auto take = [&](int64_t bytes) { char* r = base + at; at += (bytes + 255) / 256 * 256; return r; };
     const int T = p.split ? 2 : 1;
@@ -96,6 +99,15 @@ template <class T> static void run(const hipadj_orthogonal* o, const Plan& p, co
     io.g_b = o->grad_stride[0]; io.g_r = o->grad_stride[1]; io.m_b = o->momentum_stride[0]; io.m_r = o->momentum_stride[1]; io.o_b = o->out_stride[0]; io.o_r = o->out_stride[1];
     io.beta = (float)o->beta; io.scale = (float)o->scale; io.nesterov = o->nesterov;
     io.vec = (uintptr_t)out % (4 * sizeof(T)) == 0 && io.o_r % 4 == 0 && (o->batch == 1 || io.o_b % 4 == 0);
+    if (p.small) {
+        Coefficients co;
+        for (int i = 0; i < 3 * o->steps; ++i) co.c[i] = (float)o->coefficients[i];
+        const dim3 grid((uint32_t)o->batch);
+        if (p.q.n <= 32) k_small<T, 32><<<grid, dim3(64), 0, s>>>(io, p.q.m, p.q.n, p.q.flip, o->steps, co);
+        else if (p.q.n <= 64) k_small<T, 64><<<grid, dim3(256), 0, s>>>(io, p.q.m, p.q.n, p.q.flip, o->steps, co);
+        else k_small<T, 128><<<grid, dim3(1024), 0, s>>>(io, p.q.m, p.q.n, p.q.flip, o->steps, co);
+        return;
+    }
     if (p.split) iterate<T, true>(o, p.q, io, s);
     else if constexpr (sizeof(T) == 2) iterate<T, false>(o, p.q, io, s);
 }
@@ -127,7 +139,7 @@ static int check(const hipadj_orthogonal* o) {
     if (!o || o->struct_size != sizeof(hipadj_orthogonal)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonal.struct_size does not match this library");
     if (o->dtype != HIPADJ_F32 && o->dtype != HIPADJ_BF16 && o->dtype != HIPADJ_F16) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: matrices are F32, BF16 or F16");
     if (o->batch < 0 || o->rows < 0 || o->cols < 0) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: negative size");
-    if (o->steps < 1 || o->steps > 64 || !o->coefficients) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: 1 to 64 steps with three coefficients each, got %d", o->steps);
+    if (o->steps < 1 || o->steps > MOST_STEPS || !o->coefficients) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: 1 to 64 steps with three coefficients each, got %d", o->steps);
     for (int i = 0; i < 3 * o->steps; ++i)
         if (!(std::fabs(o->coefficients[i]) <= 32.0)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: coefficients within +-32, got %g", o->coefficients[i]);
     double s, big;
@@ -151,8 +163,8 @@ extern "C" int hipadj_orthogonalized_update_dev(const hipadj_orthogonal* o, cons
     const int rc = orth::check(o);
     if (rc != HIPADJ_OK) return rc;
     if (o->batch == 0 || o->rows == 0 || o->cols == 0) return HIPADJ_OK;
-    if (!grad || !out || !workspace || (uintptr_t)workspace % 256) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonalized_update_dev: grad, out and a 256-byte aligned workspace are required");
     const orth::Plan p = orth::plan_of(o, (char*)workspace);
+    if (!grad || !out || (p.bytes && (!workspace || (uintptr_t)workspace % 256))) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonalized_update_dev: grad, out and a 256-byte aligned workspace are required");
     OpsDevice dev(o->device);
     if (dev.rc != HIPADJ_OK) return dev.rc;
     hipStream_t s = (hipStream_t)stream;

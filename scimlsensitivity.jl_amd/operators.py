@@ -267,6 +267,6 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     L = _lib.load()
     ws = C.c_int64()
     _check(L.hipadj_orthogonalized_update_size(C.byref(q), C.byref(ws)))
-    work = torch.empty(ws.value, dtype=torch.uint8, device=grad.device)
+    work = torch.empty(ws.value, dtype=torch.uint8, device=grad.device) if ws.value else None
     _check(L.hipadj_orthogonalized_update_dev(C.byref(q), _ptr(g), _ptr(m), _ptr(o), _ptr(work), _stream(torch, grad.device)))
     return given_out if given_out is not None else out

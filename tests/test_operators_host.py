@@ -80,7 +80,8 @@ def test_orthogonal_arguments(lib):
     _lib, L = lib
     o = orthogonal(_lib)
     assert L.hipadj_orthogonalized_update_dev(C.byref(o), None, None, 256, 256, None) == -1
-    assert L.hipadj_orthogonalized_update_dev(C.byref(o), 256, None, 256, 128, None) == -1 and b"aligned" in L.hipadj_last_error(None)
+    large = orthogonal(_lib, rows=400)
+    assert L.hipadj_orthogonalized_update_dev(C.byref(large), 256, None, 256, 128, None) == -1 and b"aligned" in L.hipadj_last_error(None)
     assert L.hipadj_orthogonalized_update_dev(C.byref(orthogonal(_lib, rows=0)), None, None, None, None, None) == 0
 
 
