@@ -173,11 +173,15 @@ __device__ inline uint64_t across(uint64_t v, int quad) {
     return (uint64_t)lo1 << 32 | lo0;
 }
 
-template <class T, int BT, int EPI, bool SPLIT>
-__global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Product g, const Mat q, const Io<T> io, const int from, const int to) {
+// SLOTS: slices of a stage and factor — the two terms of a split factor, whose three products then share what is read; or two neighbouring slices of K, which halves the number of stages
+// where the tile is so small that each stage costs the latency of memory; or one.
+template <class T, int BT, int EPI, bool SPLIT, int SLOTS>
+__global__ void __launch_bounds__(256, BT == 64 || (BT == 128 && SLOTS == 1) ? 2 : 1) k_product(const Product g, const Mat q, const Io<T> io, const int from, const int to) {
     constexpr int W = BT / 64;                // 32 x 32 accumulators a wave and direction
     constexpr int RQ = BT / 64;               // requests of a wave, factor and stage
-    __shared__ __align__(16) f16 s0[2 * BT * BK], s1[2 * BT * BK], s2[2 * BT * BK], s3[2 * BT * BK];
+    constexpr int SLICE = BT * BK, BUF = 2 * SLOTS * SLICE;   // P's slices, then Q's
+    static_assert(!SPLIT || SLOTS == 2, "a slot for each term");
+    __shared__ __align__(16) f16 s0[BUF], s1[BUF], s2[BUF], s3[BUF];
     const int64_t b = blockIdx.z;
     int bi, bj;
     if constexpr (EPI == GRAM || EPI == POLY) {               // tile t of the lower triangle
@@ -203,7 +207,8 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
         for (int y = 0; y < W; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-    const int per = (int)(g.K / BK), stages = SPLIT ? 3 * per : per;              // multiples of four
+    constexpr int DEPTH = SPLIT ? BK : SLOTS * BK;            // of a stage, in k
+    const int stages = (int)(g.K / DEPTH);                    // a multiple of four, or of two
     // rows past the last one (the sides are multiples of 128, not of every BT) are requested from the last one, multiplied and not stored
     int64_t row_p[RQ], row_q[RQ];
 #pragma unroll
@@ -212,65 +217,78 @@ __global__ void __launch_bounds__(256, BT == 256 ? 1 : 2) k_product(const Produc
         row_p[c] = (i0 + r < g.M ? i0 + r : g.M - 1) * g.K + k;
         row_q[c] = (j0 + r < g.N ? j0 + r : g.N - 1) * g.K + k;
     }
-    // requests n of the 2 RQ of a stage; behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
+    // request n of the 2 SLOTS RQ of a stage; behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
+    constexpr int NREQ = 2 * SLOTS * RQ;
     auto request = [&](int s, f16* buf, int n) {
         s = s < stages ? s : stages - 1;
-        const int part = SPLIT ? s / per : 0, k = (SPLIT ? s % per : s) * BK, c = n % RQ;
-        const f16* from = n < RQ ? g.P[SPLIT && part == 2 ? 1 : 0] + b * g.sP + k + row_p[c] : g.Q[SPLIT && part == 1 ? 1 : 0] + b * g.sQ + k + row_q[c];
+        const int slice = n / RQ, c = n % RQ, slot = slice % SLOTS, term = SPLIT ? slot : 0;
+        const int k = s * DEPTH + (SPLIT ? 0 : slot * BK);
+        const f16* from = slice < SLOTS ? g.P[term] + b * g.sP + k + row_p[c] : g.Q[term] + b * g.sQ + k + row_q[c];
         __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                         (__attribute__((address_space(3))) void*)(buf + (n < RQ ? 0 : BT * BK) + (wave * RQ + c) * 512), 16, 0, 0);
+                                         (__attribute__((address_space(3))) void*)(buf + slice * SLICE + (wave * RQ + c) * 512), 16, 0, 0);
     };
-    const int rp = (wi * (BT / 2) + (lane & 31)) * BK, rq = BT * BK + (wj * (BT / 2) + (lane & 31)) * BK;
+    const int rp = (wi * (BT / 2) + (lane & 31)) * BK, rq = SLOTS * SLICE + (wj * (BT / 2) + (lane & 31)) * BK;
     const int ch0 = ((lane >> 5) ^ ((lane >> 2) & 3)) * 8, ch1 = ((2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 8;
-    f16x8 p0[W], q0[W], p1[W], q1[W];
-    auto read = [&](const f16* buf, int ch, f16x8 (&fp)[W], f16x8 (&fq)[W], int n) {      // n of the 2 W factors
-        if (n < W) fp[n] = *(const f16x8*)(buf + rp + n * 32 * BK + ch);
-        else fq[n - W] = *(const f16x8*)(buf + rq + (n - W) * 32 * BK + ch);
+    typedef f16x8 Factors[SLOTS][2][W];                       // [slot][P, Q]
+    constexpr int NREAD = 2 * SLOTS * W;
+    Factors f0, f1;
+    auto read = [&](const f16* buf, int ch, Factors& f, int n) {
+        const int slot = n / (2 * W), which = n / W % 2, x = n % W;
+        f[slot][which][x] = *(const f16x8*)(buf + slot * SLICE + (which ? rq : rp) + x * 32 * BK + ch);
     };
-    // half a stage: the products of one half with the reads of the next and RQ requests between them, one at a time — issued in a burst they hold the wave, and with it the matrix
-    // core, up to the rate of the request queue and of LDS
-    auto half = [&](const f16x8 (&fp)[W], const f16x8 (&fq)[W], const f16* rbuf, int ch, f16x8 (&np)[W], f16x8 (&nq)[W], int rs, f16* qbuf, int n0) {
+    // half a stage: the products of one half with the reads of the next and half a stage's requests between them, one at a time — issued in a burst they hold the wave, and with it the
+    // matrix core, up to the rate of the request queue and of LDS
+    constexpr int SETS = SPLIT ? 3 : SLOTS, NM = SETS * W * W;
+    auto half = [&](const Factors& f, const f16* rbuf, int ch, Factors& nf, int rs, f16* qbuf, int n0) {
         int reads = 0, requests = 0;
 #pragma unroll
-        for (int m = 0; m < W * W; ++m) {
-            const int x = m / W, y = m % W;
-            acc[x][y] = mfma(fp[x], fq[y], acc[x][y]);
+        for (int m = 0; m < NM; ++m) {
+            const int set = m / (W * W), x = m / W % W, y = m % W;
+            const int tp = SPLIT ? set == 1 : set, tq = SPLIT ? set == 0 : set;    // split: hi lo, lo hi, hi hi
+            acc[x][y] = mfma(f[tp][0][x], f[tq][1][y], acc[x][y]);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (; reads < 2 * W && reads * W <= (m + 1) * 3 - 1; ++reads) read(rbuf, ch, np, nq, reads);     // all within the first two thirds
-            if (requests < RQ && (m + 1) * RQ >= (requests + 1) * W * W) { request(rs, qbuf, n0 + requests); ++requests; }
+            for (; reads < NREAD && reads * 2 * NM < (m + 1) * NREAD * 3; ++reads) read(rbuf, ch, nf, reads);     // all within the first two thirds
+#pragma unroll
+            for (; requests < NREQ / 2 && (requests + 1) * NM <= (m + 1) * (NREQ / 2); ++requests) request(rs, qbuf, n0 + requests);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    // the oldest stage in flight has arrived in this wave's part (those of two later ones, 2 RQ requests each, may still be on the way) and its LDS reads are done; then in all waves
+    // the oldest stage in flight has arrived in this wave's part (those of two later ones may still be on the way) and its LDS reads are done; then in all waves
     auto arrive = [&]() {
-        static_assert(RQ >= 2 && RQ <= 4, "the counts below");
-        __builtin_amdgcn_s_waitcnt(RQ == 4 ? 0x4070 : RQ == 3 ? 0x007c : 0x0078);  // vmcnt(4 RQ) lgkmcnt(0)
+        static_assert(NREQ == 4 || NREQ == 6 || NREQ == 8, "the counts below");
+        __builtin_amdgcn_s_waitcnt(NREQ == 8 ? 0x4070 : NREQ == 6 ? 0x007c : 0x0078);        // vmcnt(2 NREQ) lgkmcnt(0)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
     };
     // behind the barrier no wave reads `now` any more: its next stage is requested half there, half in the first half of the next stage
     auto stage = [&](int s, f16* prev, f16* now, const f16* next) {
-        half(p0, q0, now, ch1, p1, q1, s + 3, prev, RQ);
+        half(f0, now, ch1, f1, s + 3, prev, NREQ / 2);
         arrive();
-        half(p1, q1, next, ch0, p0, q0, s + 4, now, 0);
+        half(f1, next, ch0, f0, s + 4, now, 0);
     };
     auto all = [&](int s, f16* buf, int from, int to) {
 #pragma unroll
         for (int n = from; n < to; ++n) request(s, buf, n);
     };
-    all(0, s0, 0, 2 * RQ); all(1, s1, 0, 2 * RQ); all(2, s2, 0, 2 * RQ);
+    all(0, s0, 0, NREQ); all(1, s1, 0, NREQ); all(2, s2, 0, NREQ);
     __builtin_amdgcn_sched_barrier(0);
     arrive();
-    all(3, s3, 0, RQ);
+    all(3, s3, 0, NREQ / 2);
 #pragma unroll
-    for (int n = 0; n < 2 * W; ++n) read(s0, ch0, p0, q0, n);
-    for (int s = 0; s < stages; s += 4) {
+    for (int n = 0; n < NREAD; ++n) read(s0, ch0, f0, n);
+    int s = 0;
+    for (; s + 4 <= stages; s += 4) {
         stage(s, s3, s0, s1);
         stage(s + 1, s0, s1, s2);
         stage(s + 2, s1, s2, s3);
         stage(s + 3, s2, s3, s0);
     }
+    if constexpr (SLOTS == 2 && !SPLIT)                       // K is a multiple of 128: two stages of 64 may be left
+        if (s < stages) {
+            stage(s, s3, s0, s1);
+            stage(s + 1, s0, s1, s2);
+        }
     __builtin_amdgcn_s_waitcnt(0x0070);                       // nothing is on the way to LDS when the workgroup ends
     // A lane holds, of each 32 x 32, column lane & 31 and rows 8 g + 4 (lane >> 5) + 0..3 for g = 0..3: four neighbours of the transposed order.  For the other order four lanes
     // exchange theirs, so that both are stored eight bytes at a time.  What a row of accumulators needs from memory is requested before any of it is used.

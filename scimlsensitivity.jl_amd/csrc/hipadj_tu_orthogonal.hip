@@ -47,24 +47,39 @@ static int64_t tiles_of(const Product& g, int64_t batch, bool lower, int64_t BT)
     const int64_t ti = (g.M + BT - 1) / BT, tj = (g.N + BT - 1) / BT;
     return (lower ? ti * (ti + 1) / 2 : ti * tj) * batch;
 }
-template <class T, int BT, int EPI, bool SPLIT> static void product(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
+template <class T, int BT, int EPI, bool SPLIT, int SLOTS> static void product(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
     const dim3 grid((uint32_t)tiles_of(g, 1, EPI == GRAM || EPI == POLY, BT), 1, (uint32_t)q.batch);
-    k_product<T, BT, EPI, SPLIT><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
+    k_product<T, BT, EPI, SPLIT, SLOTS><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
 }
 
-// The tile of a product: the one whose rounds over the 256 CUs take the least.  Measured, nanoseconds a row of K: a 256 tile 31, a 192 tile 19, a 128 tile 9.5, two of which share a CU (20).
-// Larger tiles read less LDS a product, smaller ones leave fewer CUs without work: 4096 x 4096 by symmetric halves is 253 tiles of 192 (one round), 136 of 256, 528 of 128.
+// The time of a product by tiles of BT, microseconds: rounds over the 256 CUs, each with a fixed part (first requests, epilogue) and one for every row of K, which grows with the share
+// of the CUs at work (they share L2 and power).  Fitted to 12 shapes from 256 x 256 to 4096 x 4096 with every tile, within 15 % where the choice is between near ones.  Larger tiles read
+// less a product, smaller ones leave fewer CUs without work: 4096 x 4096 takes 253 tiles of 192 for a symmetric product (87 us; 528 of 128: 119, 136 of 256: 117) and 256 of 256 for
+// B X (147; of 192: 167), 512 x 512 takes tiles of 64 (5 us; of 128: 9, of 256: 27).
+struct TileCost { int BT; double fixed, round, row, load; };
+static constexpr TileCost ONE_TERM[] = {{64, 2.0, 2.2, 3.0e-3, 0.5}, {128, 2.0, 3.5, 6.0e-3, 0.65}, {192, 3.0, 8.0, 9.8e-3, 0.9}, {256, 4.0, 14.0, 16.3e-3, 0.9}};
+static constexpr TileCost TWO_TERMS[] = {{64, 2.0, 2.5, 7.5e-3, 0.2}, {128, 3.0, 7.5, 13.0e-3, 0.5}};
+template <int N> static int best_tile(const TileCost (&table)[N], const Product& g, int64_t batch, bool lower) {
+    int best = 0;
+    double least = 0;
+    for (const TileCost& c : table) {
+        const int64_t n = tiles_of(g, batch, lower, c.BT), rounds = (n + 255) / 256;
+        const double t = c.fixed + (double)rounds * (c.round + (double)g.K * c.row * (1.0 + c.load * (double)n / (256.0 * (double)rounds)));
+        if (!best || t < least) { best = c.BT; least = t; }
+    }
+    return best;
+}
 template <class T, int EPI, bool SPLIT> static void product_of(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
-    auto cost = [&](int64_t BT) -> double {
-        const int64_t n = tiles_of(g, q.batch, EPI == GRAM || EPI == POLY, BT);
-        if (BT != 128) return (double)((n + 255) / 256) * (BT == 256 ? 31.0 : 19.0);
-        const int64_t left = n % 512;
-        return (double)(n / 512) * 20.0 + (left > 256 ? 20.0 : left ? 9.5 : 0.0);
-    };
-    const double c128 = cost(128), c192 = cost(192), c256 = cost(256);
-    if (c256 <= c192 && c256 <= c128) product<T, 256, EPI, SPLIT>(g, q, io, from, to, s);
-    else if (c192 <= c128) product<T, 192, EPI, SPLIT>(g, q, io, from, to, s);
-    else product<T, 128, EPI, SPLIT>(g, q, io, from, to, s);
+    constexpr bool LOWER = EPI == GRAM || EPI == POLY;
+    if constexpr (SPLIT) {
+        if (best_tile(TWO_TERMS, g, q.batch, LOWER) == 64) product<T, 64, EPI, true, 2>(g, q, io, from, to, s);
+        else product<T, 128, EPI, true, 2>(g, q, io, from, to, s);
+    } else switch (best_tile(ONE_TERM, g, q.batch, LOWER)) {
+        case 64: product<T, 64, EPI, false, 2>(g, q, io, from, to, s); break;
+        case 128: product<T, 128, EPI, false, 1>(g, q, io, from, to, s); break;
+        case 192: product<T, 192, EPI, false, 1>(g, q, io, from, to, s); break;
+        default: product<T, 256, EPI, false, 1>(g, q, io, from, to, s); break;
+    }
 }
 
 template <class T, bool SPLIT> static void iterate(const hipadj_orthogonal* o, const Mat& q, const Io<T>& io, hipStream_t s) {
