@@ -30,7 +30,8 @@ def _ptr(t):
 
 
 def _stream(torch, device):
-    return torch.cuda.current_stream(device).cuda_stream
+    """The hipStream_t of torch's current stream (as torch.cuda.current_stream(device).cuda_stream, without the Stream object: 0.1 of 2 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _on(name, t, like, dtype=None, shape=None):
@@ -104,7 +105,7 @@ def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
     r.gate, r.coupled, r.batch, r.length, r.channels, r.nseq = GATES[form], int(bool(coupled)), batch, length, channels, nseq
     if packed:
         r.offsets, r.offsets_bits = offsets.data_ptr(), 64 if offsets.dtype == torch.int64 else 32
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = torch.empty_like(x)
     r.x_stride[:], r.gate_stride[:], r.h_stride[:] = _strides(x, packed), _strides(gate, packed), _strides(h, packed)
     L = _lib.load()
     ck, ws = C.c_int64(), C.c_int64()
@@ -195,7 +196,7 @@ def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=No
     elif state.shape[0] < x.shape[0]:
         raise ValueError(f"{x.shape[0]} rows without slots need as many states, got {state.shape[0]}")
     x, gate = _rows(x), _rows(gate)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    h = torch.empty_like(x, memory_format=torch.contiguous_format)
     _check(_lib.load().hipadj_recurrence_step_dev(x.device.index, _DTYPES[x.dtype], _DTYPES[gate.dtype], GATES[form], bool(coupled), x.shape[0], x.shape[1], x.data_ptr(), x.stride(0),
                                                   gate.data_ptr(), gate.stride(0), state.data_ptr(), state.stride(0), state.shape[0], _ptr(slots),
                                                   64 if slots is not None and slots.dtype == torch.int64 else 32, h.data_ptr(), h.stride(0), _stream(torch, x.device)))
