@@ -50,23 +50,31 @@ template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 // ---- values -----------------------------------------------------------------------------------------------------------------------------------------------------
 
+// FAST: where x and gate have 16 bits, exp(g) is exp2(g log2 e) with the product rounded: off by |g| 2^-24 of itself, which is nothing where exp(g) is not nothing.  The states that leave
+// in 32 bits stay as exact; only a gradient with respect to a strongly negative gate is less so, and that is rounded to 16 bits.
+//
 // exp in 32 bits: exp2 of g log2(e) with the product's rounding error carried along, so that strong decays keep their digits; beyond +-200 (0 or inf in 32 bits) the argument is
 // cut off, which also keeps the error term finite for a gate of -inf or of its type's lowest value.  NaN stays NaN.
-__device__ inline float exp_(float g) {
+template <bool FAST> __device__ inline float exp_(float g) {
+    if constexpr (FAST) return __builtin_amdgcn_exp2f(g * 1.44269504f);
     g = g < -200.f ? -200.f : (g > 200.f ? 200.f : g);
     const float p = g * 1.44269504f;
     const float e = fmaf(g, 1.44269504f, -p) + g * 1.92596299e-8f;
     const float r = __builtin_amdgcn_exp2f(p);
     return fmaf(r, e * 0.693147181f, r);
 }
-__device__ inline double exp_(double g) { return exp(g); }
-// 1 - exp(g) without the cancellation at small |g| (Taylor series; the first term left out is below 2e-8 of the value at 0.35)
-__device__ inline float one_minus_exp(float g, float a) {
-    float s = fmaf(g, 1.f / 5040.f, 1.f / 720.f);
+template <bool FAST> __device__ inline double exp_(double g) { return exp(g); }
+// exp(g) and 1 - exp(g), the latter without the cancellation at small |g| (Taylor series; the first term left out is below 2e-8 of the value at 0.35, FAST: 5e-8 at 0.25)
+template <bool FAST> __device__ inline void exp_rest(float g, float& a, float& rest) {
+    a = exp_<FAST>(g);
+    float s;
+    s = FAST ? 1.f / 720.f : fmaf(g, 1.f / 5040.f, 1.f / 720.f);
     s = fmaf(s, g, 1.f / 120.f); s = fmaf(s, g, 1.f / 24.f); s = fmaf(s, g, 1.f / 6.f); s = fmaf(s, g, 0.5f); s = fmaf(s, g, 1.f);
-    return fabsf(g) < 0.35f ? -g * s : 1.f - a;
+    const bool near = fabsf(g) < (FAST ? 0.25f : 0.35f);
+    rest = near ? -g * s : 1.f - a;
+    a = near ? 1.f - rest : a;
 }
-__device__ inline double one_minus_exp(double g, double) { return -expm1(g); }
+template <bool FAST> __device__ inline void exp_rest(double g, double& a, double& rest) { a = exp(g); rest = -expm1(g); }
 __device__ inline float recip(float x) { return __builtin_amdgcn_rcpf(x); }
 __device__ inline double recip(double x) { return 1.0 / x; }
 __device__ inline float neg_abs(float x) { return -fabsf(x); }
@@ -74,12 +82,10 @@ __device__ inline double neg_abs(double x) { return -fabs(x); }
 
 // a and 1 - a of a gate; `rest` is only formed where it is used.  A decay next to one acts over hundreds of rows, so its last bit counts: where 1 - a is the smaller one it is formed
 // first, with its own relative accuracy, and a as its difference from one, within half a unit of the last place.
-template <int FORM, bool REST, class S> __device__ inline void decay(S g, S& a, S& rest) {
+template <int FORM, bool REST, bool FAST, class S> __device__ inline void decay(S g, S& a, S& rest) {
     if constexpr (FORM == 0) { a = g; if constexpr (REST) rest = S(1) - g; }
-    else if constexpr (FORM == 1) {
-        a = exp_(g);
-        if constexpr (REST) { rest = one_minus_exp(g, a); a = fabs(g) < S(0.35) ? S(1) - rest : a; }
-    } else { const S e = exp_(neg_abs(g)), s = e * recip(S(1) + e), l = S(1) - s; a = g >= S(0) ? l : s; if constexpr (REST) rest = g >= S(0) ? s : l; }
+    else if constexpr (FORM == 1) { if constexpr (REST) exp_rest<FAST>(g, a, rest); else a = exp_<FAST>(g); }
+    else { const S e = exp_<FAST>(neg_abs(g)), s = e * recip(S(1) + e), l = S(1) - s; a = g >= S(0) ? l : s; if constexpr (REST) rest = g >= S(0) ? s : l; }
 }
 
 // ---- published words ----------------------------------------------------------------------------------------------------------------------------------------------
@@ -179,7 +185,7 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             const uint32_t q = sh.cut[w];
             cut |= q;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { H[v] = through(sh.A[w][ch + v], sh.H[w][ch + v], q, H[v]); A[v] = q ? S(0) : A[v] * sh.A[w][ch + v]; }
+            for (int v = 0; v < V; ++v) { H[v] = through(sh.A[w][ch + v], sh.H[w][ch + v], q, H[v]); A[v] *= sh.A[w][ch + v]; }
         }
         if (!closes) {                                        // (only later tiles of the same group read it)
             uint64_t* dst = p.agg + (c * p.ntiles + k) * (2 * W) * CW + ch;
@@ -234,7 +240,9 @@ template <class S, int V> __device__ inline void take(const Args& p, Lds<S, V>& 
     c = t % (uint32_t)p.nchains; k = (int)(t / (uint32_t)p.nchains);
 }
 
-template <class T, int V> __device__ inline Pack<T, V> read(const void* base, int64_t at) { return *(const Pack<T, V>*)((const T*)base + at); }
+// A row is addressed by a wave-uniform base and a 32-bit byte offset of the lane: the row's part of the address is scalar arithmetic.
+template <class T, int V> __device__ inline Pack<T, V> read(const T* row, uint32_t lane_bytes) { return *(const Pack<T, V>*)((const char*)row + lane_bytes); }
+template <class T, int V> __device__ inline void write(T* row, uint32_t lane_bytes, const Pack<T, V>& v) { *(Pack<T, V>*)((char*)row + lane_bytes) = v; }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------------------------------
 
@@ -242,59 +250,79 @@ template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED
 __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Args p) {
     __shared__ Lds<S, V> sh;
     constexpr int CW = 64 * V, TS = TSF;
+    constexpr bool FAST = sizeof(T) == 2 && sizeof(TG) == 2;
     int64_t c; int k;
     take(p, sh, c, k);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t b = c / p.ncg, cg = c % p.ncg, ch = cg * CW + lane * V;
+    const int64_t b = c / p.ncg, c0 = c % p.ncg * CW, ch = c0 + lane * V;
     const bool on = ch < p.D;
-    const int64_t cl = on ? ch : 0;                           // lanes past the last channel read the first one and write nothing
+    const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T), lg = lv * sizeof(TG);      // lanes past the last channel read the first one and write nothing
+    const int64_t cl = c0 + lv;
     const int64_t t0 = (int64_t)k * TTF + wave * TS;
-    const int64_t xo = b * p.x_sb + t0 * p.x_st + cl, go = b * p.g_sb + t0 * p.g_st + cl;
-    S a[TS][V], u[TS][V];                                     // (a, b) of each row
-    Marks m{0, 0, 0};
-    if constexpr (PACKED) m = marks_of<TS>(p, t0);
-    const bool whole = t0 + TS <= p.L;
+    const int rows = (int)(p.L - t0 < TS ? (p.L > t0 ? p.L - t0 : 0) : TS);                // of this piece
+    const T* xr = (const T*)p.x + (b * p.x_sb + t0 * p.x_st + c0);
+    const TG* gr = (const TG*)p.gate + (b * p.g_sb + t0 * p.g_st + c0);
     Pack<T, V> rx[TS]; Pack<TG, V> rg[TS];
-    if (whole) {
+    if (rows == TS) {
 #pragma unroll
-        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
+        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt); }
     } else {
 #pragma unroll
-        for (int i = 0; i < TS; ++i) if (t0 + i < p.L) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
+        for (int i = 0; i < TS; ++i) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { rg[i].v[v] = (TG)S(0); rx[i].v[v] = (T)S(0); }
+            if (i < rows) { rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt); }
+        }
     }
-    S A[V], H[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+    Marks m{0, 0, 0};
+    if constexpr (PACKED) m = marks_of<TS>(p, t0);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
+    S a[TS][V], u[TS][V];                                     // (a, b) of each row
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-        const bool in = whole || t0 + i < p.L;
-        S s0[V];
-        if constexpr (PACKED) {
+    for (int i = 0; i < TS; ++i)
 #pragma unroll
-            for (int v = 0; v < V; ++v) s0[v] = S(0);
+        for (int v = 0; v < V; ++v) {
+            S rest = S(0);
+            decay<FORM, COUPLED, FAST, S>((S)rg[i].v[v], a[i][v], rest);
+            u[i][v] = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
+        }
+    if (rows < TS) {                                          // rows behind the end pass a state on
+#pragma unroll
+        for (int i = 0; i < TS; ++i) if (i >= rows) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { a[i][v] = S(1); u[i][v] = S(0); }
+        }
+    }
+    if constexpr (PACKED) if (cuts) {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
             if ((m.start >> i) & 1) {
                 const int64_t s = seq_behind(p, t0 + i);
                 if (p.h0 && s < p.nseq) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) s0[v] = ((const S*)p.h0)[s * p.D + cl + v];
+                    for (int v = 0; v < V; ++v) u[i][v] += a[i][v] * ((const S*)p.h0)[s * p.D + cl + v];
+                } else {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) u[i][v] += a[i][v] * S(0);
                 }
             }
-        }
+            if ((m.out >> i) & 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            S rest = S(0);
-            if (in) {
-                decay<FORM, COUPLED, S>((S)rg[i].v[v], a[i][v], rest);
-                u[i][v] = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
-            } else { a[i][v] = S(1); u[i][v] = S(0); }
-            if constexpr (PACKED) {
-                if ((m.start >> i) & 1) u[i][v] += a[i][v] * s0[v];
-                if ((m.out >> i) & 1) u[i][v] = S(0);
-                if ((cuts >> i) & 1) { A[v] = S(0); H[v] = u[i][v]; } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + u[i][v]; }
-            } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + u[i][v]; }
+                for (int v = 0; v < V; ++v) u[i][v] = S(0);
+            }
         }
     }
+    S A[V], H[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+#pragma unroll
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const bool cut = PACKED && ((cuts >> i) & 1);
+            H[v] = cut ? u[i][v] : a[i][v] * H[v] + u[i][v];
+            A[v] *= a[i][v];                                  // not used where the piece is cut
+        }
 #pragma unroll
     for (int v = 0; v < V; ++v) { sh.A[wave][lane * V + v] = A[v]; sh.H[wave][lane * V + v] = H[v]; }
     if (lane == 0) sh.cut[wave] = cuts != 0;
@@ -311,17 +339,16 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 #pragma unroll
         for (int v = 0; v < V; ++v) ((S*)p.ckpt)[(b * p.nckpt + t0 / TTA) * p.D + ch + v] = st[v];
     }
-    const int64_t ho = b * p.h_sb + t0 * p.h_st + ch;
+    T* hr = (T*)p.h + (b * p.h_sb + t0 * p.h_st + c0);
 #pragma unroll
     for (int i = 0; i < TS; ++i) {
+        Pack<T, V> o;
 #pragma unroll
-        for (int v = 0; v < V; ++v) st[v] = (PACKED && ((cuts >> i) & 1)) ? u[i][v] : a[i][v] * st[v] + u[i][v];
-        if (on && (whole || t0 + i < p.L)) {
-            Pack<T, V> o;
-#pragma unroll
-            for (int v = 0; v < V; ++v) o.v[v] = (T)st[v];
-            *(Pack<T, V>*)((T*)p.h + ho + i * p.h_st) = o;
+        for (int v = 0; v < V; ++v) {
+            st[v] = (PACKED && ((cuts >> i) & 1)) ? u[i][v] : a[i][v] * st[v] + u[i][v];
+            o.v[v] = (T)st[v];
         }
+        if (on && i < rows) write<T, V>(hr + i * p.h_st, lt, o);
         if constexpr (PACKED) {
             if ((m.end >> i) & 1) {
                 const int64_t s = seq_behind(p, t0 + i);
@@ -345,73 +372,95 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 }
 
 // ---- adjoint ------------------------------------------------------------------------------------------------------------------------------------------------------
-
+// Where 1 - a is needed, 16-bit data keep it in registers and a = 1 - (1 - a) is one instruction; wider ones keep a and evaluate the gate again at the end.
 template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
 __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Args p) {
     __shared__ Lds<S, V> sh;
     constexpr int CW = 64 * V, TS = TSA;
-    constexpr bool REST = COUPLED || FORM == 2;
+    constexpr bool FAST = sizeof(T) == 2 && sizeof(TG) == 2, REST = COUPLED || FORM == 2, KEEP = REST && FAST;
     int64_t c; int k;
     take(p, sh, c, k);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t b = c / p.ncg, cg = c % p.ncg, ch = cg * CW + lane * V;
+    const int64_t b = c / p.ncg, c0 = c % p.ncg * CW, ch = c0 + lane * V;
     const bool on = ch < p.D;
-    const int64_t cl = on ? ch : 0;
+    const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T), lg = lv * sizeof(TG);
+    const int64_t cl = c0 + lv;
     const int tile = p.ntiles - 1 - k;                        // the scan runs from the end: position 0 is the last tile
     const int64_t t0 = (int64_t)tile * TTA + wave * TS;
-    const int64_t xo = b * p.x_sb + t0 * p.x_st + cl, go = b * p.g_sb + t0 * p.g_st + cl, dho = b * p.dh_sb + t0 * p.dh_st + cl;
-    const bool whole = t0 + TS <= p.L;
+    const int rows = (int)(p.L - t0 < TS ? (p.L > t0 ? p.L - t0 : 0) : TS);
+    const T* xr = (const T*)p.x + (b * p.x_sb + t0 * p.x_st + c0);
+    const TG* gr = (const TG*)p.gate + (b * p.g_sb + t0 * p.g_st + c0);
+    const T* dr = (const T*)p.dh + (b * p.dh_sb + t0 * p.dh_st + c0);
     Pack<T, V> rx[TS], rd[TS]; Pack<TG, V> rg[TS];
-    if (whole) {
+    if (rows == TS && p.dh) {
 #pragma unroll
-        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
-    } else {
-#pragma unroll
-        for (int i = 0; i < TS; ++i) if (t0 + i < p.L) { rg[i] = read<TG, V>(p.gate, go + i * p.g_st); rx[i] = read<T, V>(p.x, xo + i * p.x_st); }
-    }
-    if (whole && p.dh) {
-#pragma unroll
-        for (int i = 0; i < TS; ++i) rd[i] = read<T, V>(p.dh, dho + i * p.dh_st);
+        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt); rd[i] = read<T, V>(dr + i * p.dh_st, lt); }
     } else {
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
-            if (p.dh && t0 + i < p.L) rd[i] = read<T, V>(p.dh, dho + i * p.dh_st);
-            else {
 #pragma unroll
-                for (int v = 0; v < V; ++v) rd[i].v[v] = (T)S(0);
+            for (int v = 0; v < V; ++v) { rg[i].v[v] = (TG)S(0); rx[i].v[v] = rd[i].v[v] = (T)S(0); }
+            if (i < rows) {
+                rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt);
+                if (p.dh) rd[i] = read<T, V>(dr + i * p.dh_st, lt);
             }
         }
     }
     Marks m{0, 0, 0};
     if constexpr (PACKED) m = marks_of<TS>(p, t0);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
-    S a[TS][V], before[TS][V];                                // a of each row; first its b, then the state before it
+    S kept[TS][V], before[TS][V];                             // 1 - a (KEEP) or a of each row; first its b, then the state before it
+    auto a = [&](int i, int v) -> S { return KEEP ? S(1) - kept[i][v] : kept[i][v]; };
+    auto at_seq = [&](const void* of, int i, int v) -> S {    // of the sequence that row i belongs to, in h0 or dh_final
+        const int64_t s = seq_behind(p, t0 + i);
+        return of && s < p.nseq ? ((const S*)of)[s * p.D + cl + v] : S(0);
+    };
+    // the cotangent of a row's state from outside the recurrence (a sequence's last row also feeds its final state); nothing in a row of no sequence
+    auto cot = [&](int i, int v) -> S {
+        S d = (S)rd[i].v[v];
+        if constexpr (PACKED) {
+            if ((m.out >> i) & 1) d = S(0);
+            if ((m.end >> i) & 1) d += at_seq(p.dh_final, i, v);
+        }
+        return d;
+    };
+#pragma unroll
+    for (int i = 0; i < TS; ++i)
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            S aa, rest = S(0);
+            decay<FORM, REST, FAST, S>((S)rg[i].v[v], aa, rest);
+            kept[i][v] = KEEP ? rest : aa;
+            before[i][v] = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
+        }
+    if (rows < TS) {                                          // rows behind the end pass a state on
+#pragma unroll
+        for (int i = 0; i < TS; ++i) if (i >= rows) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) { kept[i][v] = KEEP ? S(0) : S(1); before[i][v] = S(0); }
+        }
+    }
+    if constexpr (PACKED) if (m.out) {
+#pragma unroll
+        for (int i = 0; i < TS; ++i) if ((m.out >> i) & 1) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) before[i][v] = S(0);
+        }
+    }
+    // the rows' forward map, for the states
     S A[V], H[V], F[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
-    auto at_seq = [&](const void* rows, int i, int v) -> S {  // row of the sequence that row i belongs to, in h0 or dh_final
-        const int64_t s = seq_behind(p, t0 + i);
-        return rows && s < p.nseq ? ((const S*)rows)[s * p.D + cl + v] : S(0);
-    };
-    // the rows' forward map, for the states
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-        const bool in = whole || t0 + i < p.L;
+    for (int i = 0; i < TS; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            S rest = S(0), bb = S(0);
-            if (in) {
-                decay<FORM, COUPLED, S>((S)rg[i].v[v], a[i][v], rest);
-                bb = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
-            } else a[i][v] = S(1);
-            if constexpr (PACKED) { if ((m.out >> i) & 1) bb = S(0); }
-            before[i][v] = bb;
-            if constexpr (PACKED) {
-                if ((m.start >> i) & 1) bb += a[i][v] * at_seq(p.h0, i, v);
-                if ((cuts >> i) & 1) { A[v] = S(0); H[v] = bb; } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + bb; }
-            } else { A[v] *= a[i][v]; H[v] = a[i][v] * H[v] + bb; }
+            const S ai = a(i, v);
+            S bb = before[i][v];
+            if constexpr (PACKED) { if ((m.start >> i) & 1) bb += ai * at_seq(p.h0, i, v); }
+            H[v] = (PACKED && ((cuts >> i) & 1)) ? bb : ai * H[v] + bb;
+            A[v] *= ai;
         }
-    }
 #pragma unroll
     for (int v = 0; v < V; ++v) { sh.A[wave][lane * V + v] = A[v]; sh.H[wave][lane * V + v] = H[v]; }
     if (lane == 0) sh.cut[wave] = cuts != 0;
@@ -424,22 +473,13 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
         for (int v = 0; v < V; ++v) F[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, F[v]);
     }
     __syncthreads();
-    // the cotangent of a row's state from outside the recurrence (a sequence's last row also feeds its final state); nothing in a row of no sequence
-    auto cot = [&](int i, int v) -> S {
-        S d = (S)rd[i].v[v];
-        if constexpr (PACKED) {
-            if ((m.out >> i) & 1) d = S(0);
-            if ((m.end >> i) & 1) d += at_seq(p.dh_final, i, v);
-        }
-        return d;
-    };
     // the rows' reverse map R -> A R + H with the same product A
 #pragma unroll
     for (int v = 0; v < V; ++v) H[v] = S(0);
 #pragma unroll
     for (int i = TS - 1; i >= 0; --i) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) { const S d = cot(i, v); H[v] = (PACKED && ((cuts >> i) & 1)) ? S(0) : a[i][v] * (d + H[v]); }
+        for (int v = 0; v < V; ++v) { const S d = cot(i, v); H[v] = (PACKED && ((cuts >> i) & 1)) ? S(0) : a(i, v) * (d + H[v]); }
     }
     const int rw = NW - 1 - wave;                             // the piece's place in scan order
 #pragma unroll
@@ -462,34 +502,32 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
             if (PACKED && ((m.start >> i) & 1)) F[v] = at_seq(p.h0, i, v);
             const S bb = before[i][v];
             before[i][v] = F[v];
-            F[v] = a[i][v] * F[v] + bb;
+            F[v] = a(i, v) * F[v] + bb;
             if (PACKED && ((m.out >> i) & 1)) F[v] = S(0);
         }
     }
-    const int64_t dxo = b * p.dx_sb + t0 * p.dx_st + ch, dgo = b * p.dg_sb + t0 * p.dg_st + ch;
+    T* dxr = (T*)p.dx + (b * p.dx_sb + t0 * p.dx_st + c0);
+    TG* dgr = (TG*)p.dgate + (b * p.dg_sb + t0 * p.dg_st + c0);
 #pragma unroll
     for (int i = TS - 1; i >= 0; --i) {
-        const bool in = whole || t0 + i < p.L;
         Pack<T, V> ox; Pack<TG, V> og;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const S G = cot(i, v) + R[v];
-            S aa = a[i][v], rest = S(1), x = S(0);
-            if (in) {
-                if constexpr (REST) decay<FORM, true, S>((S)rg[i].v[v], aa, rest);
-                if constexpr (COUPLED) x = (S)rx[i].v[v];
-            }
-            S da = G * (before[i][v] - x);
-            if constexpr (FORM == 1) da *= a[i][v];
-            if constexpr (FORM == 2) da *= a[i][v] * rest;
+            const S G = cot(i, v) + R[v], ai = a(i, v);
+            S aa, rest = S(1);
+            if constexpr (KEEP) rest = kept[i][v];
+            else if constexpr (REST) decay<FORM, true, FAST, S>((S)rg[i].v[v], aa, rest);
+            S da = G * (COUPLED ? before[i][v] - (S)rx[i].v[v] : before[i][v]);
+            if constexpr (FORM == 1) da *= ai;
+            if constexpr (FORM == 2) da *= ai * rest;
             S dx = COUPLED ? G * rest : G;
-            R[v] = a[i][v] * G;
+            R[v] = ai * G;
             if (PACKED && ((m.out >> i) & 1)) { da = S(0); dx = S(0); R[v] = S(0); }
             ox.v[v] = (T)dx; og.v[v] = (TG)da;
         }
-        if (on && in) {
-            if (p.dx) *(Pack<T, V>*)((T*)p.dx + dxo + i * p.dx_st) = ox;
-            if (p.dgate) *(Pack<TG, V>*)((TG*)p.dgate + dgo + i * p.dg_st) = og;
+        if (on && i < rows) {
+            if (p.dx) write<T, V>(dxr + i * p.dx_st, lt, ox);
+            if (p.dgate) write<TG, V>(dgr + i * p.dg_st, lg, og);
         }
         if constexpr (PACKED) {
             if ((m.start >> i) & 1) {
@@ -557,13 +595,13 @@ __global__ void __launch_bounds__(NS) k_step(const StepArgs p, int ncg) {
     }
     for (int64_t i = r; i < p.B; ++i) {
         if (i != r) { if (!more) break; if (slot_of(i) != slot) continue; }
-        const Pack<T, V> x = read<T, V>(p.x, i * p.x_s + ch);
-        const Pack<TG, V> g = read<TG, V>(p.gate, i * p.g_s + ch);
+        const Pack<T, V> x = *(const Pack<T, V>*)((const T*)p.x + i * p.x_s + ch);
+        const Pack<TG, V> g = *(const Pack<TG, V>*)((const TG*)p.gate + i * p.g_s + ch);
         Pack<T, V> o;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             S a, rest = S(0);
-            decay<FORM, COUPLED, S>((S)g.v[v], a, rest);
+            decay<FORM, COUPLED, sizeof(T) == 2 && sizeof(TG) == 2, S>((S)g.v[v], a, rest);
             st[v] = a * st[v] + (COUPLED ? rest * (S)x.v[v] : (S)x.v[v]);
             o.v[v] = (T)st[v];
         }
