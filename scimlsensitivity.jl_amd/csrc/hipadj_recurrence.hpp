@@ -193,10 +193,12 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             for (int v = 0; v < V; ++v) { publish(dst + v, CW, A[v], cut ? TAG_CUT : TAG_MAP); publish(dst + W * CW + v, CW, H[v], TAG_MAP); }
         }
     }
-    S st[V];
+    // the maps of the group's earlier tiles, NW at a time, one a wave; composed to (B, G)
+    S B[V], G[V];
+    uint32_t gcut = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) st[v] = first[v];
-    for (int j0 = 0; j0 == 0 || j0 < before; j0 += NW) {
+    for (int v = 0; v < V; ++v) { B[v] = S(1); G[v] = S(0); }
+    for (int j0 = 0; j0 < before; j0 += NW) {
         const int j = j0 + wave;
         if (j < before) {
             const uint64_t* src = p.agg + (c * p.ntiles + base + j) * (2 * W) * CW + ch;
@@ -205,86 +207,118 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             for (int v = 0; v < V; ++v) { q = await_value(src + v, CW, sh.pA[wave][ch + v]); await_value(src + W * CW + v, CW, sh.pH[wave][ch + v]); }
             if (lane == 0) sh.pcut[wave] = q == TAG_CUT;
         }
-        if (j0 == 0 && g > 0 && wave == (before < NW ? before : NW - 1)) {
-            const uint64_t* src = p.car + (c * ngroups + g) * W * CW + ch;
-#pragma unroll
-            for (int v = 0; v < V; ++v) await_value(src + v, CW, sh.c[ch + v]);
-        }
         __syncthreads();
-        if (j0 == 0 && g > 0) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) st[v] = sh.c[ch + v];
-        }
         for (int i = 0; i < NW && j0 + i < before; ++i) {
             const uint32_t q = sh.pcut[i];
+            gcut |= q;
 #pragma unroll
-            for (int v = 0; v < V; ++v) st[v] = through(sh.pA[i][ch + v], sh.pH[i][ch + v], q, st[v]);
+            for (int v = 0; v < V; ++v) { G[v] = through(sh.pA[i][ch + v], sh.pH[i][ch + v], q, G[v]); B[v] *= sh.pA[i][ch + v]; }
         }
-        if (j0 + NW < before) __syncthreads();                // the next NW maps take the same place
+        __syncthreads();
     }
-    if (wave == 0 && closes) {
-        uint64_t* dst = p.car + (c * ngroups + g + 1) * W * CW + ch;
+    // the state at the group's start: wave 0 waits for it and, in the group's last tile, has the next group's on its way two operations later
+    if (g > 0) {
+        if (wave == 0) {
+            const uint64_t* src = p.car + (c * ngroups + g) * W * CW + ch;
+            uint64_t* dst = p.car + (c * ngroups + g + 1) * W * CW + ch;
 #pragma unroll
-        for (int v = 0; v < V; ++v) publish(dst + v, CW, through(A[v], H[v], cut, st[v]), TAG_MAP);
+            for (int v = 0; v < V; ++v) {
+                S s;
+                await_value(src + v, CW, s);
+                if (closes) publish(dst + v, CW, through(A[v], H[v], cut, through(B[v], G[v], gcut, s)), TAG_MAP);
+                sh.c[ch + v] = s;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int v = 0; v < V; ++v) carry[v] = through(B[v], G[v], gcut, sh.c[ch + v]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            carry[v] = through(B[v], G[v], gcut, first[v]);
+            if (wave == 0 && closes) publish(p.car + (c * ngroups + g + 1) * W * CW + ch + v, CW, through(A[v], H[v], cut, carry[v]), TAG_MAP);
+        }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v) carry[v] = st[v];
 }
 
-// the tile of this workgroup: chain and position in scan order
-template <class S, int V> __device__ inline void take(const Args& p, Lds<S, V>& sh, int64_t& c, int& k) {
-    if (p.ntiles == 1) { c = blockIdx.x; k = 0; return; }
-    if (threadIdx.x == 0) sh.ticket = atomicAdd(p.ticket, 1u);
+// The tile of this workgroup.  Tile t: chain t % nchains, position t / nchains in scan order.  (Workgroups that stay and request the next tile's inputs while they wait for a state were
+// slower: a tile that is taken early and begun late holds up its chain; 226 us against 201 for one sequence of 65536 rows.)
+__device__ inline uint32_t take(const Args& p, uint32_t* slot) {
+    if (p.ntiles == 1) return blockIdx.x;
+    if (threadIdx.x == 0) *slot = atomicAdd(p.ticket, 1u);
     __syncthreads();
-    const uint32_t t = __builtin_amdgcn_readfirstlane(sh.ticket);
-    c = t % (uint32_t)p.nchains; k = (int)(t / (uint32_t)p.nchains);
+    return __builtin_amdgcn_readfirstlane(*slot);
 }
 
 // A row is addressed by a wave-uniform base and a 32-bit byte offset of the lane: the row's part of the address is scalar arithmetic.
-template <class T, int V> __device__ inline Pack<T, V> read(const T* row, uint32_t lane_bytes) { return *(const Pack<T, V>*)((const char*)row + lane_bytes); }
+// What is on its way stays one integer a lane (two 16-bit values split up would take two registers), and `arrived` keeps the compiler from splitting it, and so waiting for it, where it
+// is requested instead of where it is used.
+template <int BYTES> struct Bits;
+template <> struct Bits<2> { typedef uint16_t memory; typedef uint32_t type; };
+template <> struct Bits<4> { typedef uint32_t memory, type; };
+template <> struct Bits<8> { typedef uint64_t memory, type; };
+template <class T, int V> using Raw = typename Bits<sizeof(T) * V>::type;
+template <class T, int V> using RawMemory = typename Bits<sizeof(T) * V>::memory;
+template <class T, int V> __device__ inline Raw<T, V> read(const T* row, uint32_t lane_bytes) { return *(const RawMemory<T, V>*)((const char*)row + lane_bytes); }
+template <class T, int V> __device__ inline T part(Raw<T, V> r, int v) { return __builtin_bit_cast(Pack<T, V>, (RawMemory<T, V>)r).v[v]; }
+template <class R, int N> __device__ inline void arrived(R (&r)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(r[i]));
+}
 template <class T, int V> __device__ inline void write(T* row, uint32_t lane_bytes, const Pack<T, V>& v) { *(Pack<T, V>*)((char*)row + lane_bytes) = v; }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------------------------------------------
 
+// where a piece of a tile lies
+struct Piece { int64_t b, c0, t0; int k, rows, channels; };
+template <int V, int TS> __device__ inline Piece piece_of(const Args& p, uint32_t tile, int wave, bool backwards) {
+    Piece q;
+    const uint32_t c = tile % (uint32_t)p.nchains;
+    q.k = (int)(tile / (uint32_t)p.nchains);
+    q.b = c / (uint32_t)p.ncg; q.c0 = (int64_t)(c % (uint32_t)p.ncg) * (64 * V);
+    q.channels = (int)(p.D - q.c0 < 64 * V ? p.D - q.c0 : 64 * V);
+    q.t0 = (int64_t)(backwards ? p.ntiles - 1 - q.k : q.k) * (NW * TS) + wave * TS;
+    q.rows = (int)(p.L - q.t0 < TS ? (p.L > q.t0 ? p.L - q.t0 : 0) : TS);
+    return q;
+}
+// the piece's rows of one input; behind the end the last row again (L > 0), which nothing uses
+template <class T, int V, int TS> __device__ inline void fetch(const Args& p, const void* base, int64_t sb, int64_t st, const Piece& q, uint32_t lane_bytes, Raw<T, V> (&r)[TS]) {
+    const int64_t t = q.t0 < p.L ? q.t0 : p.L - 1;
+    const T* row = (const T*)base + (q.b * sb + t * st + q.c0);
+#pragma unroll
+    for (int i = 0; i < TS; ++i) {
+        r[i] = read<T, V>(row, lane_bytes);
+        row += i + 1 < q.rows ? st : 0;                       // (stepped: TS multiples of st would be kept, and spilled, across the tiles)
+    }
+}
+
 template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
 __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Args p) {
     __shared__ Lds<S, V> sh;
-    constexpr int CW = 64 * V, TS = TSF;
+    constexpr int TS = TSF;
     constexpr bool FAST = sizeof(T) == 2 && sizeof(TG) == 2;
-    int64_t c; int k;
-    take(p, sh, c, k);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t b = c / p.ncg, c0 = c % p.ncg * CW, ch = c0 + lane * V;
-    const bool on = ch < p.D;
-    const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T), lg = lv * sizeof(TG);      // lanes past the last channel read the first one and write nothing
-    const int64_t cl = c0 + lv;
-    const int64_t t0 = (int64_t)k * TTF + wave * TS;
-    const int rows = (int)(p.L - t0 < TS ? (p.L > t0 ? p.L - t0 : 0) : TS);                // of this piece
-    const T* xr = (const T*)p.x + (b * p.x_sb + t0 * p.x_st + c0);
-    const TG* gr = (const TG*)p.gate + (b * p.g_sb + t0 * p.g_st + c0);
-    Pack<T, V> rx[TS]; Pack<TG, V> rg[TS];
-    if (rows == TS) {
-#pragma unroll
-        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt); }
-    } else {
-#pragma unroll
-        for (int i = 0; i < TS; ++i) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) { rg[i].v[v] = (TG)S(0); rx[i].v[v] = (T)S(0); }
-            if (i < rows) { rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt); }
-        }
-    }
+    const uint32_t tile = take(p, &sh.ticket);
+    const Piece q = piece_of<V, TS>(p, tile, wave, false);
+    const int64_t b = q.b, c = tile % (uint32_t)p.nchains, t0 = q.t0, c0 = q.c0;
+    const int k = q.k, rows = q.rows;
+    const bool on = lane * V < q.channels;
+    const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T);     // lanes past the last channel read the first one and write nothing
+    Raw<T, V> rx[TS]; Raw<TG, V> rg[TS];
+    fetch<TG, V, TS>(p, p.gate, p.g_sb, p.g_st, q, lv * sizeof(TG), rg);
+    fetch<T, V, TS>(p, p.x, p.x_sb, p.x_st, q, lt, rx);
     Marks m{0, 0, 0};
     if constexpr (PACKED) m = marks_of<TS>(p, t0);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
+    arrived(rg); arrived(rx);
     S a[TS][V], u[TS][V];                                     // (a, b) of each row
 #pragma unroll
     for (int i = 0; i < TS; ++i)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             S rest = S(0);
-            decay<FORM, COUPLED, FAST, S>((S)rg[i].v[v], a[i][v], rest);
-            u[i][v] = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
+            decay<FORM, COUPLED, FAST, S>((S)part<TG, V>(rg[i], v), a[i][v], rest);
+            u[i][v] = COUPLED ? rest * (S)part<T, V>(rx[i], v) : (S)part<T, V>(rx[i], v);
         }
     if (rows < TS) {                                          // rows behind the end pass a state on
 #pragma unroll
@@ -300,7 +334,7 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
                 const int64_t s = seq_behind(p, t0 + i);
                 if (p.h0 && s < p.nseq) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) u[i][v] += a[i][v] * ((const S*)p.h0)[s * p.D + cl + v];
+                    for (int v = 0; v < V; ++v) u[i][v] += a[i][v] * ((const S*)p.h0 + (s * p.D + c0))[lv + v];
                 } else {
 #pragma unroll
                     for (int v = 0; v < V; ++v) u[i][v] += a[i][v] * S(0);
@@ -328,16 +362,16 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
     if (lane == 0) sh.cut[wave] = cuts != 0;
     S first[V], st[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) first[v] = (!PACKED && p.h0) ? ((const S*)p.h0)[b * p.D + cl + v] : S(0);
+    for (int v = 0; v < V; ++v) first[v] = (!PACKED && p.h0) ? ((const S*)p.h0 + (b * p.D + c0))[lv + v] : S(0);
     chain<S, V>(p, sh, c, k, first, st);
     for (int w = 0; w < wave; ++w) {
-        const uint32_t q = sh.cut[w];
+        const uint32_t z = sh.cut[w];
 #pragma unroll
-        for (int v = 0; v < V; ++v) st[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, st[v]);
+        for (int v = 0; v < V; ++v) st[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], z, st[v]);
     }
     if (p.ckpt && on && wave * TS % TTA == 0 && t0 / TTA < p.nckpt) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) ((S*)p.ckpt)[(b * p.nckpt + t0 / TTA) * p.D + ch + v] = st[v];
+        for (int v = 0; v < V; ++v) ((S*)p.ckpt + ((b * p.nckpt + t0 / TTA) * p.D + c0))[lv + v] = st[v];
     }
     T* hr = (T*)p.h + (b * p.h_sb + t0 * p.h_st + c0);
 #pragma unroll
@@ -348,13 +382,14 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
             st[v] = (PACKED && ((cuts >> i) & 1)) ? u[i][v] : a[i][v] * st[v] + u[i][v];
             o.v[v] = (T)st[v];
         }
-        if (on && i < rows) write<T, V>(hr + i * p.h_st, lt, o);
+        if (on && i < rows) write<T, V>(hr, lt, o);
+        hr += p.h_st;
         if constexpr (PACKED) {
             if ((m.end >> i) & 1) {
                 const int64_t s = seq_behind(p, t0 + i);
                 if (on && s < p.nseq) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) ((S*)p.h_final)[s * p.D + ch + v] = st[v];
+                    for (int v = 0; v < V; ++v) ((S*)p.h_final + (s * p.D + c0))[lv + v] = st[v];
                 }
             }
         }
@@ -363,11 +398,11 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
         for (int64_t s = (int64_t)k * NW + wave; s < p.nseq; s += (int64_t)p.ntiles * NW)
             if (offset_at(p, s + 1) <= offset_at(p, s) && on) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) ((S*)p.h_final)[s * p.D + ch + v] = p.h0 ? ((const S*)p.h0)[s * p.D + ch + v] : S(0);
+                for (int v = 0; v < V; ++v) ((S*)p.h_final + (s * p.D + c0))[lv + v] = p.h0 ? ((const S*)p.h0 + (s * p.D + c0))[lv + v] : S(0);
             }
-    } else if (on && k == p.ntiles - 1 && (p.L ? (t0 <= p.L - 1 && t0 + TS > p.L - 1) : wave == 0)) {
+    } else if (on && k == p.ntiles - 1 && t0 <= p.L - 1 && t0 + TS > p.L - 1) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) ((S*)p.h_final)[b * p.D + ch + v] = st[v];
+        for (int v = 0; v < V; ++v) ((S*)p.h_final + (b * p.D + c0))[lv + v] = st[v];
     }
 }
 
@@ -376,48 +411,36 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
 __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Args p) {
     __shared__ Lds<S, V> sh;
-    constexpr int CW = 64 * V, TS = TSA;
+    constexpr int TS = TSA;
     constexpr bool FAST = sizeof(T) == 2 && sizeof(TG) == 2, REST = COUPLED || FORM == 2, KEEP = REST && FAST;
-    int64_t c; int k;
-    take(p, sh, c, k);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int64_t b = c / p.ncg, c0 = c % p.ncg * CW, ch = c0 + lane * V;
-    const bool on = ch < p.D;
+    const uint32_t taken = take(p, &sh.ticket);
+    const Piece q = piece_of<V, TS>(p, taken, wave, true);
+    const int64_t b = q.b, c = taken % (uint32_t)p.nchains, t0 = q.t0, c0 = q.c0;
+    const int k = q.k, rows = q.rows, tile = p.ntiles - 1 - k;      // the scan runs from the end: position 0 is the last tile
+    const bool on = lane * V < q.channels;
     const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T), lg = lv * sizeof(TG);
-    const int64_t cl = c0 + lv;
-    const int tile = p.ntiles - 1 - k;                        // the scan runs from the end: position 0 is the last tile
-    const int64_t t0 = (int64_t)tile * TTA + wave * TS;
-    const int rows = (int)(p.L - t0 < TS ? (p.L > t0 ? p.L - t0 : 0) : TS);
-    const T* xr = (const T*)p.x + (b * p.x_sb + t0 * p.x_st + c0);
-    const TG* gr = (const TG*)p.gate + (b * p.g_sb + t0 * p.g_st + c0);
-    const T* dr = (const T*)p.dh + (b * p.dh_sb + t0 * p.dh_st + c0);
-    Pack<T, V> rx[TS], rd[TS]; Pack<TG, V> rg[TS];
-    if (rows == TS && p.dh) {
+    Raw<T, V> rx[TS], rd[TS]; Raw<TG, V> rg[TS];
+    fetch<TG, V, TS>(p, p.gate, p.g_sb, p.g_st, q, lg, rg);
+    fetch<T, V, TS>(p, p.x, p.x_sb, p.x_st, q, lt, rx);
+    if (p.dh) fetch<T, V, TS>(p, p.dh, p.dh_sb, p.dh_st, q, lt, rd);
+    else {
 #pragma unroll
-        for (int i = 0; i < TS; ++i) { rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt); rd[i] = read<T, V>(dr + i * p.dh_st, lt); }
-    } else {
-#pragma unroll
-        for (int i = 0; i < TS; ++i) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) { rg[i].v[v] = (TG)S(0); rx[i].v[v] = rd[i].v[v] = (T)S(0); }
-            if (i < rows) {
-                rg[i] = read<TG, V>(gr + i * p.g_st, lg); rx[i] = read<T, V>(xr + i * p.x_st, lt);
-                if (p.dh) rd[i] = read<T, V>(dr + i * p.dh_st, lt);
-            }
-        }
+        for (int i = 0; i < TS; ++i) rd[i] = 0;
     }
     Marks m{0, 0, 0};
     if constexpr (PACKED) m = marks_of<TS>(p, t0);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
+    arrived(rg); arrived(rx); arrived(rd);
     S kept[TS][V], before[TS][V];                             // 1 - a (KEEP) or a of each row; first its b, then the state before it
     auto a = [&](int i, int v) -> S { return KEEP ? S(1) - kept[i][v] : kept[i][v]; };
     auto at_seq = [&](const void* of, int i, int v) -> S {    // of the sequence that row i belongs to, in h0 or dh_final
         const int64_t s = seq_behind(p, t0 + i);
-        return of && s < p.nseq ? ((const S*)of)[s * p.D + cl + v] : S(0);
+        return of && s < p.nseq ? ((const S*)of + (s * p.D + c0))[lv + v] : S(0);
     };
     // the cotangent of a row's state from outside the recurrence (a sequence's last row also feeds its final state); nothing in a row of no sequence
     auto cot = [&](int i, int v) -> S {
-        S d = (S)rd[i].v[v];
+        S d = (S)part<T, V>(rd[i], v);
         if constexpr (PACKED) {
             if ((m.out >> i) & 1) d = S(0);
             if ((m.end >> i) & 1) d += at_seq(p.dh_final, i, v);
@@ -429,13 +452,14 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             S aa, rest = S(0);
-            decay<FORM, REST, FAST, S>((S)rg[i].v[v], aa, rest);
+            decay<FORM, REST, FAST, S>((S)part<TG, V>(rg[i], v), aa, rest);
             kept[i][v] = KEEP ? rest : aa;
-            before[i][v] = COUPLED ? rest * (S)rx[i].v[v] : (S)rx[i].v[v];
+            before[i][v] = COUPLED ? rest * (S)part<T, V>(rx[i], v) : (S)part<T, V>(rx[i], v);
         }
     if (rows < TS) {                                          // rows behind the end pass a state on
 #pragma unroll
         for (int i = 0; i < TS; ++i) if (i >= rows) {
+            rd[i] = 0;
 #pragma unroll
             for (int v = 0; v < V; ++v) { kept[i][v] = KEEP ? S(0) : S(1); before[i][v] = S(0); }
         }
@@ -466,11 +490,11 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
     if (lane == 0) sh.cut[wave] = cuts != 0;
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < V; ++v) F[v] = ((const S*)p.ckpt)[(b * p.nckpt + tile) * p.D + cl + v];
+    for (int v = 0; v < V; ++v) F[v] = ((const S*)p.ckpt + ((b * p.nckpt + tile) * p.D + c0))[lv + v];
     for (int w = 0; w < wave; ++w) {
-        const uint32_t q = sh.cut[w];
+        const uint32_t z = sh.cut[w];
 #pragma unroll
-        for (int v = 0; v < V; ++v) F[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, F[v]);
+        for (int v = 0; v < V; ++v) F[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], z, F[v]);
     }
     __syncthreads();
     // the rows' reverse map R -> A R + H with the same product A
@@ -487,13 +511,14 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
     if (lane == 0) sh.cut[rw] = cuts != 0;
     S first[V], R[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) first[v] = (!PACKED && p.dh_final) ? ((const S*)p.dh_final)[b * p.D + cl + v] : S(0);
+    for (int v = 0; v < V; ++v) first[v] = (!PACKED && p.dh_final) ? ((const S*)p.dh_final + (b * p.D + c0))[lv + v] : S(0);
     chain<S, V>(p, sh, c, k, first, R);
     for (int w = 0; w < rw; ++w) {
-        const uint32_t q = sh.cut[w];
+        const uint32_t z = sh.cut[w];
 #pragma unroll
-        for (int v = 0; v < V; ++v) R[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], q, R[v]);
+        for (int v = 0; v < V; ++v) R[v] = through(sh.A[w][lane * V + v], sh.H[w][lane * V + v], z, R[v]);
     }
+    arrived(rx); arrived(rd);                                 // (their 32-bit forms are made again, not kept)
     // the states before each row, then the rows from the last to the first
 #pragma unroll
     for (int i = 0; i < TS; ++i) {
@@ -506,8 +531,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
             if (PACKED && ((m.out >> i) & 1)) F[v] = S(0);
         }
     }
-    T* dxr = (T*)p.dx + (b * p.dx_sb + t0 * p.dx_st + c0);
-    TG* dgr = (TG*)p.dgate + (b * p.dg_sb + t0 * p.dg_st + c0);
+    T* dxr = (T*)p.dx + (b * p.dx_sb + (t0 + TS - 1) * p.dx_st + c0);
+    TG* dgr = (TG*)p.dgate + (b * p.dg_sb + (t0 + TS - 1) * p.dg_st + c0);
 #pragma unroll
     for (int i = TS - 1; i >= 0; --i) {
         Pack<T, V> ox; Pack<TG, V> og;
@@ -516,8 +541,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
             const S G = cot(i, v) + R[v], ai = a(i, v);
             S aa, rest = S(1);
             if constexpr (KEEP) rest = kept[i][v];
-            else if constexpr (REST) decay<FORM, true, FAST, S>((S)rg[i].v[v], aa, rest);
-            S da = G * (COUPLED ? before[i][v] - (S)rx[i].v[v] : before[i][v]);
+            else if constexpr (REST) decay<FORM, true, FAST, S>((S)part<TG, V>(rg[i], v), aa, rest);
+            S da = G * (COUPLED ? before[i][v] - (S)part<T, V>(rx[i], v) : before[i][v]);
             if constexpr (FORM == 1) da *= ai;
             if constexpr (FORM == 2) da *= ai * rest;
             S dx = COUPLED ? G * rest : G;
@@ -526,15 +551,16 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
             ox.v[v] = (T)dx; og.v[v] = (TG)da;
         }
         if (on && i < rows) {
-            if (p.dx) write<T, V>(dxr + i * p.dx_st, lt, ox);
-            if (p.dgate) write<TG, V>(dgr + i * p.dg_st, lg, og);
+            if (p.dx) write<T, V>(dxr, lt, ox);
+            if (p.dgate) write<TG, V>(dgr, lg, og);
         }
+        dxr -= p.dx_st; dgr -= p.dg_st;
         if constexpr (PACKED) {
             if ((m.start >> i) & 1) {
                 const int64_t s = seq_behind(p, t0 + i);
                 if (on && p.dh0 && s < p.nseq) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) ((S*)p.dh0)[s * p.D + ch + v] = R[v];
+                    for (int v = 0; v < V; ++v) ((S*)p.dh0 + (s * p.D + c0))[lv + v] = R[v];
                 }
 #pragma unroll
                 for (int v = 0; v < V; ++v) R[v] = S(0);
@@ -545,11 +571,11 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_adjoint(const Ar
         for (int64_t s = (int64_t)k * NW + wave; s < p.nseq; s += (int64_t)p.ntiles * NW)
             if (offset_at(p, s + 1) <= offset_at(p, s) && on && p.dh0) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) ((S*)p.dh0)[s * p.D + ch + v] = p.dh_final ? ((const S*)p.dh_final)[s * p.D + ch + v] : S(0);
+                for (int v = 0; v < V; ++v) ((S*)p.dh0 + (s * p.D + c0))[lv + v] = p.dh_final ? ((const S*)p.dh_final + (s * p.D + c0))[lv + v] : S(0);
             }
     } else if (on && tile == 0 && wave == 0 && p.dh0) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) ((S*)p.dh0)[b * p.D + ch + v] = R[v];
+        for (int v = 0; v < V; ++v) ((S*)p.dh0 + (b * p.D + c0))[lv + v] = R[v];
     }
 }
 

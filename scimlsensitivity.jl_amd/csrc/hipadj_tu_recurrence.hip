@@ -1,4 +1,5 @@
 // hipadj_tu_recurrence.hip — translation units of the gated linear recurrence: hipcc -DHIPADJ_TU_PAIR=<rec::PAIR_*>; without it the C entry points.
+#include <algorithm>
 #include "hipadj_recurrence.hpp"
 
 #if defined(HIPADJ_TU_PAIR)
@@ -44,7 +45,6 @@ template void launch_step<HIPADJ_TU_PAIR>(const StepArgs&, bool, int, bool, hipS
 
 }  // namespace rec
 #else
-#include <algorithm>
 #include <cstdio>
 #include "../../include/hipadj.h"
 #include "hipadj_ops.hpp"
@@ -54,6 +54,11 @@ namespace rec {
 // the words of the chains and the ticket, zeroed before the launch that uses them
 static __global__ void __launch_bounds__(256) k_zero(uint64_t* w, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) w[i] = 0;
+}
+
+// no rows: what leaves is what came in
+template <class S> static __global__ void __launch_bounds__(256) k_same(S* to, const S* from, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) to[i] = from ? from[i] : S(0);
 }
 
 static int pair_of(int dtype, int gate_dtype) {
@@ -121,6 +126,15 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
     const int64_t words = words_of(r, s, V);
     OpsDevice dev(r->device);
     if (dev.rc != HIPADJ_OK) return dev.rc;
+    if (r->length == 0) {
+        const int64_t n = (r->nseq ? r->nseq : r->batch) * r->channels;
+        void* to = adjoint ? a.dh0 : a.h_final;
+        const void* from = adjoint ? a.dh_final : a.h0;
+        const dim3 grid((uint32_t)std::min<int64_t>(1024, (n + 255) / 256)), block(256);
+        if (to && r->dtype == HIPADJ_F64) k_same<double><<<grid, block, 0, (hipStream_t)stream>>>((double*)to, (const double*)from, n);
+        else if (to) k_same<float><<<grid, block, 0, (hipStream_t)stream>>>((float*)to, (const float*)from, n);
+        return ops_launched("recurrence");
+    }
     if (words) {
         if (!workspace || (uintptr_t)workspace % 8) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: %lld rows need a workspace (hipadj_recurrence_sizes), 8-byte aligned", (long long)r->length);
         uint64_t* w = (uint64_t*)workspace;
@@ -159,7 +173,7 @@ extern "C" int hipadj_recurrence_adjoint_dev(const hipadj_recurrence* r, const v
     const int rc = rec::check(r);
     if (rc != HIPADJ_OK) return rc;
     if (r->channels == 0 || (r->nseq == 0 && r->batch == 0)) return HIPADJ_OK;
-    if (!checkpoints || (r->length > 0 && (!x || !gate))) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_recurrence_adjoint_dev: x, gate and the forward pass's checkpoints are required");
+    if (r->length > 0 && (!checkpoints || !x || !gate)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_recurrence_adjoint_dev: x, gate and the forward pass's checkpoints are required");
     rec::Args a{};
     a.x = x; a.gate = gate; a.h0 = h0; a.ckpt = const_cast<void*>(checkpoints); a.dh = dh; a.dh_final = dh_final; a.dx = dx; a.dgate = dgate; a.dh0 = dh0;
     return rec::go(r, a, true, workspace, stream);
