@@ -14,7 +14,7 @@
 //     GS tiles carried through the maps of the group's earlier tiles, in this fixed order — the result does not depend on which tile ran first — and the last tile of a group
 //     publishes the state at the next group's start.  A long axis therefore costs one exchange per GROUP on the critical path, not one per tile.
 // Tiles are handed out by a ticket (one atomic increment per workgroup) in an order where a tile only ever waits for tiles with lower tickets: those already run, and the
-// publication of a map waits for nothing, so every wait ends.  A published value travels in 64-bit words of 32 bits of data and a non-zero tag, written and read as relaxed
+// publication of a map waits for nothing, so every wait ends.  Published values travel in 64-bit words that also say that they are there, written and read as relaxed
 // device-scope atomics: a word is complete or absent, nothing orders one word against another and no cache has to be written back.  The words are zeroed by a launch of their own.
 //
 // The adjoint does not read h: the forward pass leaves the state at the start of every TTA rows (the checkpoints, 1 / TTA of h in 32 bits) and a tile of the adjoint re-solves its rows from there in
@@ -42,7 +42,7 @@ struct Args {
     int64_t x_sb, x_st, g_sb, g_st, h_sb, h_st, dh_sb, dh_st, dx_sb, dx_st, dg_sb, dg_st;
     int64_t L, D, nseq;
     int32_t offsets64, ntiles, nckpt, ncg, nchains, GS;      // nckpt: checkpoints of a batch row; ncg: channel groups; nchains = batch * ncg; GS: tiles of a group
-    uint64_t *agg, *car;                                     // [nchains][ntiles][2 * WPV][CW], [nchains][ngroups][WPV][CW]
+    uint64_t *agg, *car;                                     // [nchains][ntiles][WPM][CW], [nchains][ngroups][WPV][CW]
     uint32_t* ticket;
 };
 
@@ -112,7 +112,28 @@ __device__ inline uint32_t await_value(const uint64_t* w, int64_t cw, double& v)
     v = __longlong_as_double((long long)((q & 0xffffffffu) | (r << 32)));
     return (uint32_t)(q >> 32);
 }
-constexpr uint32_t TAG_MAP = 1, TAG_CUT = 2;                  // CUT: no state passes (a sequence starts inside): H alone, whatever A and the state are
+// A map (A, H); CUT: no state passes (a sequence starts inside), H alone counts, whatever A and the state are.  In 32 bits it is one word: the last bit of A is set for "present", which
+// moves A by at most 2^-23 of itself.  1 (the smallest denormal) is CUT, 3 stands for zero — a state times it is nothing, but a NaN stays one — and the largest number for infinity.
+constexpr uint32_t TAG_VALUE = 1, TAG_CUT = 2;
+template <class S> constexpr int WPM = sizeof(S) == 4 ? 1 : 4;         // words of a map
+__device__ inline void publish_map(uint64_t* w, int64_t, float A, float H, uint32_t cut) {
+    uint32_t a = __float_as_uint(A) | 1u;
+    if ((a & 0x7ffffffeu) == 0) a = 3u;
+    if ((__float_as_uint(A) & 0x7fffffffu) == 0x7f800000u) a = (__float_as_uint(A) & 0x80000000u) | 0x7f7fffffu;
+    put(w, (uint64_t(__float_as_uint(H)) << 32) | (cut ? 1u : a));
+}
+__device__ inline void publish_map(uint64_t* w, int64_t cw, double A, double H, uint32_t cut) { publish(w, cw, A, cut ? TAG_CUT : TAG_VALUE); publish(w + 2 * cw, cw, H, TAG_VALUE); }
+__device__ inline uint32_t await_map(const uint64_t* w, int64_t, float& A, float& H) {
+    uint64_t q;
+    while (!((q = get(w)) & 1u)) __builtin_amdgcn_s_sleep(1);
+    A = __uint_as_float((uint32_t)q); H = __uint_as_float((uint32_t)(q >> 32));
+    return (uint32_t)q == 1u;
+}
+__device__ inline uint32_t await_map(const uint64_t* w, int64_t cw, double& A, double& H) {
+    const uint32_t q = await_value(w, cw, A);
+    await_value(w + 2 * cw, cw, H);
+    return q == TAG_CUT;
+}
 
 // ---- packed sequences ---------------------------------------------------------------------------------------------------------------------------------------------
 
@@ -171,7 +192,7 @@ template <class S> __device__ inline S through(S A, S H, uint32_t cut, S c) { re
 // The state at the start of position `k` of chain `c` (positions are in scan order; the adjoint counts tiles from the end), given the maps of its NW pieces in sh.A / sh.H / sh.cut
 // (piece order is scan order too).  `first`: the state at the chain's start.  Publishes what later tiles of the chain wait for.  Returns with all pieces' waves past a barrier.
 template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>& sh, int64_t c, int k, const S (&first)[V], S (&carry)[V]) {
-    constexpr int CW = 64 * V, W = WPV<S>;
+    constexpr int CW = 64 * V, W = WPV<S>, WM = WPM<S>;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, ch = lane * V;
     const int g = k / p.GS, base = g * p.GS, before = k - base, ngroups = (p.ntiles + p.GS - 1) / p.GS;
     const bool last = k == p.ntiles - 1, closes = !last && before == p.GS - 1;
@@ -188,9 +209,9 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             for (int v = 0; v < V; ++v) { H[v] = through(sh.A[w][ch + v], sh.H[w][ch + v], q, H[v]); A[v] *= sh.A[w][ch + v]; }
         }
         if (!closes) {                                        // (only later tiles of the same group read it)
-            uint64_t* dst = p.agg + (c * p.ntiles + k) * (2 * W) * CW + ch;
+            uint64_t* dst = p.agg + (c * p.ntiles + k) * WM * CW + ch;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { publish(dst + v, CW, A[v], cut ? TAG_CUT : TAG_MAP); publish(dst + W * CW + v, CW, H[v], TAG_MAP); }
+            for (int v = 0; v < V; ++v) publish_map(dst + v, CW, A[v], H[v], cut);
         }
     }
     // the maps of the group's earlier tiles, NW at a time, one a wave; composed to (B, G)
@@ -201,11 +222,11 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
     for (int j0 = 0; j0 < before; j0 += NW) {
         const int j = j0 + wave;
         if (j < before) {
-            const uint64_t* src = p.agg + (c * p.ntiles + base + j) * (2 * W) * CW + ch;
+            const uint64_t* src = p.agg + (c * p.ntiles + base + j) * WM * CW + ch;
             uint32_t q = 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { q = await_value(src + v, CW, sh.pA[wave][ch + v]); await_value(src + W * CW + v, CW, sh.pH[wave][ch + v]); }
-            if (lane == 0) sh.pcut[wave] = q == TAG_CUT;
+            for (int v = 0; v < V; ++v) q = await_map(src + v, CW, sh.pA[wave][ch + v], sh.pH[wave][ch + v]);
+            if (lane == 0) sh.pcut[wave] = q;
         }
         __syncthreads();
         for (int i = 0; i < NW && j0 + i < before; ++i) {
@@ -225,7 +246,7 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             for (int v = 0; v < V; ++v) {
                 S s;
                 await_value(src + v, CW, s);
-                if (closes) publish(dst + v, CW, through(A[v], H[v], cut, through(B[v], G[v], gcut, s)), TAG_MAP);
+                if (closes) publish(dst + v, CW, through(A[v], H[v], cut, through(B[v], G[v], gcut, s)), TAG_VALUE);
                 sh.c[ch + v] = s;
             }
         }
@@ -236,7 +257,7 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             carry[v] = through(B[v], G[v], gcut, first[v]);
-            if (wave == 0 && closes) publish(p.car + (c * ngroups + g + 1) * W * CW + ch + v, CW, through(A[v], H[v], cut, carry[v]), TAG_MAP);
+            if (wave == 0 && closes) publish(p.car + (c * ngroups + g + 1) * W * CW + ch + v, CW, through(A[v], H[v], cut, carry[v]), TAG_VALUE);
         }
     }
 }

@@ -81,16 +81,15 @@ static void run(int pair, const Args& a, bool adjoint, bool wide, int form, bool
 }
 
 // the split of a problem: it depends on the sizes alone
-struct Split { int64_t ntiles, GS; };
-static Split split_of(const hipadj_recurrence* r, bool adjoint) {
-    const int64_t rows = adjoint ? TTA : TTF;
-    return {std::max<int64_t>(1, (r->length + rows - 1) / rows), NW};
-}
-// words for the narrower channel group (V = 1), which needs at least as many
-static int64_t words_of(const hipadj_recurrence* r, const Split& s, int V) {
-    if (s.ntiles == 1) return 0;
-    const int64_t CW = 64 * V, chains = r->batch * ((r->channels + CW - 1) / CW), W = r->dtype == HIPADJ_F64 ? 2 : 1;
-    return 1 + chains * CW * W * (2 * s.ntiles + (s.ntiles + s.GS - 1) / s.GS);
+static int64_t tiles_of(const hipadj_recurrence* r, bool adjoint) { const int64_t rows = adjoint ? TTA : TTF; return std::max<int64_t>(1, (r->length + rows - 1) / rows); }
+// Tiles of a group.  The exchange from group to group is what a few long chains wait for, and reading the group's earlier maps is what many chains pay for: 32 and 8.  Measured, forward:
+// 1 x 65536 x 128 BF16 (one chain) 54 us with groups of 8, 36 with 32; 1 x 65536 x 2048 (16 chains) 213 and 277; 8 x 4096 x 2048 (128 chains) 107 and 132.
+static int group_of(int64_t nchains) { return nchains <= 4 ? 32 : 8; }
+// 64-bit words of a launch: the ticket, a map for each tile, a state for each group, by channel
+static int64_t words_of(const hipadj_recurrence* r, int64_t ntiles, int V) {
+    if (ntiles == 1) return 0;
+    const int64_t CW = 64 * V, chains = r->batch * ((r->channels + CW - 1) / CW), GS = group_of(chains), wide = r->dtype == HIPADJ_F64;
+    return 1 + chains * CW * ((wide ? WPM<double> : WPM<float>) * ntiles + (wide ? WPV<double> : WPV<float>) * ((ntiles + GS - 1) / GS));
 }
 
 static int check(const hipadj_recurrence* r) {
@@ -100,9 +99,9 @@ static int check(const hipadj_recurrence* r) {
     if (r->batch < 0 || r->length < 0 || r->channels < 0 || r->nseq < 0) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: negative size");
     if (r->nseq > 0 && (r->batch != 1 || !r->offsets)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: packed sequences (nseq > 0) need batch = 1 and offsets[nseq + 1]");
     if (r->nseq > 0 && r->offsets_bits != 32 && r->offsets_bits != 64) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: offsets_bits must be 32 or 64");
-    const Split s = split_of(r, true);
+    const int64_t ntiles = tiles_of(r, true);
     const int64_t chains = r->channels ? (r->channels + 63) / 64 : 0;
-    if (r->batch && chains && s.ntiles > ((int64_t(1) << 31) - 1) / chains / r->batch) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence: more than 2^31 - 1 tiles");
+    if (r->batch && chains && ntiles > ((int64_t(1) << 31) - 1) / chains / r->batch) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence: more than 2^31 - 1 tiles");
     return HIPADJ_OK;
 }
 
@@ -113,7 +112,7 @@ static bool fits(const void* p, const int64_t* st, int64_t bytes, int64_t V) {
 static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace, void* stream) {
     const int pair = pair_of(r->dtype, r->gate_dtype);
     const int64_t xb = size_of(r->dtype), gb = size_of(r->gate_dtype), VW = xb == 2 ? 2 : 1;
-    const Split s = split_of(r, adjoint);
+    const int64_t ntiles = tiles_of(r, adjoint);
     // V neighbouring channels a lane where every row starts on a multiple of V elements; else one (odd channel counts, sliced inputs)
     const bool wide = VW == 1 || (r->channels % VW == 0 && fits(a.x, r->x_stride, xb, VW) && fits(a.gate, r->gate_stride, gb, VW) &&
                                   (adjoint ? fits(a.dh, r->dh_stride, xb, VW) && fits(a.dx, r->dx_stride, xb, VW) && fits(a.dgate, r->dgate_stride, gb, VW)
@@ -122,8 +121,8 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
     a.x_sb = r->x_stride[0]; a.x_st = r->x_stride[1]; a.g_sb = r->gate_stride[0]; a.g_st = r->gate_stride[1]; a.h_sb = r->h_stride[0]; a.h_st = r->h_stride[1];
     a.dh_sb = r->dh_stride[0]; a.dh_st = r->dh_stride[1]; a.dx_sb = r->dx_stride[0]; a.dx_st = r->dx_stride[1]; a.dg_sb = r->dgate_stride[0]; a.dg_st = r->dgate_stride[1];
     a.L = r->length; a.D = r->channels; a.nseq = r->nseq; a.offsets = r->offsets; a.offsets64 = r->offsets_bits == 64;
-    a.ntiles = (int)s.ntiles; a.nckpt = (int)split_of(r, true).ntiles; a.GS = (int)s.GS; a.ncg = (int)((r->channels + 64 * V - 1) / (64 * V)); a.nchains = (int)(r->batch * a.ncg);
-    const int64_t words = words_of(r, s, V);
+    a.ntiles = (int)ntiles; a.nckpt = (int)tiles_of(r, true); a.ncg = (int)((r->channels + 64 * V - 1) / (64 * V)); a.nchains = (int)(r->batch * a.ncg); a.GS = group_of(a.nchains);
+    const int64_t words = words_of(r, ntiles, V);
     OpsDevice dev(r->device);
     if (dev.rc != HIPADJ_OK) return dev.rc;
     if (r->length == 0) {
@@ -138,8 +137,8 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
     if (words) {
         if (!workspace || (uintptr_t)workspace % 8) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: %lld rows need a workspace (hipadj_recurrence_sizes), 8-byte aligned", (long long)r->length);
         uint64_t* w = (uint64_t*)workspace;
-        const int64_t W = r->dtype == HIPADJ_F64 ? 2 : 1;
-        a.ticket = (uint32_t*)w; a.agg = w + 1; a.car = a.agg + (int64_t)a.nchains * a.ntiles * 2 * W * 64 * V;
+        const int64_t W = r->dtype == HIPADJ_F64 ? WPM<double> : WPM<float>;
+        a.ticket = (uint32_t*)w; a.agg = w + 1; a.car = a.agg + (int64_t)a.nchains * a.ntiles * W * 64 * V;
         k_zero<<<dim3((uint32_t)std::min<int64_t>(1024, (words + 255) / 256)), dim3(256), 0, (hipStream_t)stream>>>(w, words);
     }
     run(pair, a, adjoint, wide, r->gate, r->coupled != 0, r->nseq > 0, (hipStream_t)stream);
@@ -151,9 +150,9 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
 extern "C" int hipadj_recurrence_sizes(const hipadj_recurrence* r, int64_t* checkpoint_bytes, int64_t* workspace_bytes) {
     const int rc = rec::check(r);
     if (rc != HIPADJ_OK) return rc;
-    const rec::Split s = rec::split_of(r, true);              // the adjoint's tiles are the smaller ones: its words suffice for the forward pass
-    if (checkpoint_bytes) *checkpoint_bytes = r->batch * s.ntiles * r->channels * (r->dtype == HIPADJ_F64 ? 8 : 4);
-    if (workspace_bytes) *workspace_bytes = 8 * std::max(rec::words_of(r, s, 1), rec::words_of(r, s, 2));
+    const int64_t ntiles = rec::tiles_of(r, true);            // the adjoint's tiles are the smaller ones: its words suffice for the forward pass
+    if (checkpoint_bytes) *checkpoint_bytes = r->batch * ntiles * r->channels * (r->dtype == HIPADJ_F64 ? 8 : 4);
+    if (workspace_bytes) *workspace_bytes = 8 * std::max(rec::words_of(r, ntiles, 1), rec::words_of(r, ntiles, 2));
     return HIPADJ_OK;
 }
 
