@@ -244,6 +244,44 @@ class WideDeviceFunction(DeviceFunction):
         _lib.declare_dense_chain(fun.id, w, input_power)      # hipadj_create routes (2, H, H, 2) chains with H in {32, 64, 128} to the FP64-MFMA family (csrc/hipadj_route.hpp)
         return fun
 
+    def weight_blocks(self):
+        """[(offset, out, in)] of the weights of a dense_chain model in its parameter vector: each the [out x in] matrix column-major, followed by its `out` biases."""
+        if getattr(self, "chain", None) is None:
+            raise ValueError(f"{self.name} is not a dense_chain model: its parameters are not known to be weight matrices")
+        blocks, off = [], 0
+        for inp, out in zip(self.chain[0][:-1], self.chain[0][1:]):
+            blocks.append((off, out, inp))
+            off += out * inp + out
+        return blocks
+
+    def orthogonalized_update(self, dp, momentum=None, *, beta=0.95, nesterov=True, steps=5, coefficients=None, device=0):
+        """The step of a dense_chain model's parameters after a gradient `dp` [np] of a loss (adjoint_sensitivities, Engine.adjoint_dev): every weight matrix's part is the
+        orthogonalised update (operators.orthogonalized_update) of its gradient, times max(1, out / in) ** 0.5; the biases' parts are the plain ones.  p -= lr * the result.
+        dp: a numpy array (the result is one, computed on cuda:`device`) or a GPU tensor.  momentum: float32 GPU tensor [np], updated in place (None: no momentum).
+        The weights' parts are computed in 32 bits."""
+        import torch
+        from . import operators
+        blocks = self.weight_blocks()
+        host = not isinstance(dp, torch.Tensor)
+        g = torch.as_tensor(np_.ascontiguousarray(dp), device=f"cuda:{int(device)}") if host else dp
+        if tuple(g.shape) != (self.np,):
+            raise ValueError(f"dp must have shape ({self.np},), got {tuple(g.shape)}")
+        if momentum is not None and (tuple(momentum.shape) != (self.np,) or momentum.dtype != torch.float32 or momentum.device != g.device or not momentum.is_contiguous()):
+            raise ValueError(f"momentum must be a contiguous float32 tensor ({self.np},) on {g.device}")
+        g32, out = g.float(), torch.empty(self.np, dtype=torch.float32, device=g.device)
+        for off, rows, cols in blocks:                       # column-major [rows x cols] is row-major [cols x rows], and the iteration commutes with transposition
+            at, b = slice(off, off + rows * cols), slice(off + rows * cols, off + rows * cols + rows)
+            view = lambda t: t[at].view(cols, rows)          # noqa: B023, E731
+            operators.orthogonalized_update(view(g32), None if momentum is None else view(momentum), beta=beta, nesterov=nesterov, steps=steps,
+                                            coefficients=coefficients or operators.NEWTON_SCHULZ, scale=max(1.0, rows / cols) ** 0.5, out=view(out))
+            if momentum is None:
+                out[b] = g32[b]
+            else:
+                momentum[b].mul_(beta).add_(g32[b])
+                out[b] = g32[b] + beta * momentum[b] if nesterov else momentum[b]
+        out = out.to(g.dtype)
+        return out.cpu().numpy() if host else out
+
     @classmethod
     def from_callable(cls, name, fn, n, np, threads=0, check=False, cost=None, mass_matrix=None):
         """A wide model from a host-language right-hand side written with array operations: `fn(u, p, t, ops) -> du` is traced once (wtrace.py), the recorded
