@@ -460,6 +460,7 @@ typedef enum { HIPADJ_GATE_DECAY = 0, HIPADJ_GATE_LOG = 1, HIPADJ_GATE_SIGMOID =
  *   packed  nseq > 0, batch = 1: sequence s is the rows offsets[s] <= t < offsets[s + 1] (device memory, ascending; equal neighbours: an empty sequence, whose final state is its
  *           first); h0, h_final, dh_final, dh0 [nseq][channels].  Rows of no sequence have h = 0 and zero gradients and are not used.  Offsets that do not ascend or pass `length` give
  *           unspecified results, never an access outside the arrays.
+ *           Decays above one are taken as they are; where their product over some hundred rows overflows, so may a state that row by row would not yet.
  * dtype: x, h, dh, dx; gate_dtype: gate, dgate — the same, or F32 next to BF16 / F16.  h0, h_final, dh_final, dh0 and the checkpoints: F64 for F64, else F32, contiguous.  States and
  * gradients are carried in that type, the outputs rounded once.
  *   hipadj_recurrence_sizes         bytes of the checkpoints and of the workspace (8-byte aligned; 0: none) of a configuration
@@ -483,9 +484,10 @@ typedef struct {
     int64_t x_stride[2], gate_stride[2], h_stride[2], dh_stride[2], dx_stride[2], dgate_stride[2]; /* batch, time */
 } hipadj_recurrence;
 int hipadj_recurrence_sizes(const hipadj_recurrence *r, int64_t *checkpoint_bytes, int64_t *workspace_bytes);
-int hipadj_recurrence_forward_dev(const hipadj_recurrence *r, const void *x, const void *gate, const void *h0, void *h, void *h_final, void *checkpoints, void *workspace, void *stream);
+int hipadj_recurrence_forward_dev(const hipadj_recurrence *r, const void *x, const void *gate, const void *h0, void *h, void *h_final, void *checkpoints, void *workspace,
+                                  int64_t workspace_bytes, void *stream);
 int hipadj_recurrence_adjoint_dev(const hipadj_recurrence *r, const void *x, const void *gate, const void *h0, const void *checkpoints, const void *dh, const void *dh_final,
-                                  void *dx, void *dgate, void *dh0, void *workspace, void *stream);
+                                  void *dx, void *dgate, void *dh0, void *workspace, int64_t workspace_bytes, void *stream);
 int hipadj_recurrence_step_dev(int32_t device, int32_t dtype, int32_t gate_dtype, int32_t gate_form, int32_t coupled, int64_t batch, int64_t channels, const void *x, int64_t x_stride,
                                const void *gate, int64_t gate_stride, void *state, int64_t state_stride, int64_t nslots, const void *slots, int32_t slots_bits, void *h, int64_t h_stride,
                                void *stream);
@@ -494,7 +496,9 @@ int hipadj_recurrence_step_dev(int32_t device, int32_t dtype, int32_t gate_dtype
  *   X = u / (|u|_F + 1e-7),  `steps` times  X <- c0 X + c1 A X + c2 A A X  with A = X X' (X' X when that is smaller),  out = scale X
  * — the nearest semi-orthogonal matrix up to the factors the coefficients leave (for (3.4445, -4.7750, 2.0315): singular values in 0.7 ... 1.2).  grad, out [batch][rows][cols] of dtype
  * F32, BF16 or F16, momentum the same shape in F32 (NULL: none), column stride 1, rows and matrices strided.  Arithmetic: products of two-term F16 splits (22 bits) accumulated
- * in F32; for BF16 with both sides of at least 256, one F16 term a factor, whose rounding adds about as much as the output's own.  A matrix with a non-finite entry gives NaN. */
+ * in F32; for BF16 with both sides of at least 256, one F16 term a factor, whose rounding adds about as much as the output's own.  A matrix with a non-finite entry gives NaN.
+ * Coefficients within +-32 under which no singular value can pass 6 and no eigenvalue of c1 A + c2 A A 24 (HIPADJ_ERR_UNSUPPORTED otherwise: F16 factors would overflow).  Sides up to
+ * 65536 and 32768, up to 65535 matrices.  out may be grad; momentum overlaps neither.  Sides up to 128 need no workspace, others 256-byte aligned. */
 typedef struct {
     uint32_t struct_size;      /* = sizeof(hipadj_orthogonal) */
     int32_t device, dtype, steps, nesterov, reserved;
@@ -504,7 +508,7 @@ typedef struct {
     const double *coefficients; /* host [steps][3] */
 } hipadj_orthogonal;
 int hipadj_orthogonalized_update_size(const hipadj_orthogonal *o, int64_t *workspace_bytes);
-int hipadj_orthogonalized_update_dev(const hipadj_orthogonal *o, const void *grad, float *momentum, void *out, void *workspace, void *stream);
+int hipadj_orthogonalized_update_dev(const hipadj_orthogonal *o, const void *grad, float *momentum, void *out, void *workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

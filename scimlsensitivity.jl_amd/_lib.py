@@ -166,11 +166,11 @@ def load():
     L.hipadj_device_count.restype = C.c_int
     i64, i32 = C.c_int64, C.c_int32
     L.hipadj_recurrence_sizes.argtypes = [C.POINTER(HipadjRecurrence), C.POINTER(i64), C.POINTER(i64)]
-    L.hipadj_recurrence_forward_dev.argtypes = [C.POINTER(HipadjRecurrence)] + [vp] * 8
-    L.hipadj_recurrence_adjoint_dev.argtypes = [C.POINTER(HipadjRecurrence)] + [vp] * 11
+    L.hipadj_recurrence_forward_dev.argtypes = [C.POINTER(HipadjRecurrence)] + [vp] * 7 + [i64, vp]
+    L.hipadj_recurrence_adjoint_dev.argtypes = [C.POINTER(HipadjRecurrence)] + [vp] * 10 + [i64, vp]
     L.hipadj_recurrence_step_dev.argtypes = [i32, i32, i32, i32, i32, i64, i64, vp, i64, vp, i64, vp, i64, i64, vp, i32, vp, i64, vp]
     L.hipadj_orthogonalized_update_size.argtypes = [C.POINTER(HipadjOrthogonal), C.POINTER(i64)]
-    L.hipadj_orthogonalized_update_dev.argtypes = [C.POINTER(HipadjOrthogonal)] + [vp] * 5
+    L.hipadj_orthogonalized_update_dev.argtypes = [C.POINTER(HipadjOrthogonal)] + [vp] * 4 + [i64, vp]
     _lib = L
     return L
 

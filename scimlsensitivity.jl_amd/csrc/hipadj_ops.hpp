@@ -18,6 +18,7 @@ static inline int ops_fail(int code, const char* text) { ops_set_error(text); re
 struct OpsDevice {
     int rc = HIPADJ_OK, old = -1;
     explicit OpsDevice(int device) {
+        (void)hipGetLastError();                    // of an earlier call of the host program: ops_launched reports this call's launches
         int n = 0;
         if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) { (void)hipGetLastError(); rc = ops_fail(HIPADJ_ERR_NO_DEVICE, "no usable HIP device (gfx950 required; there is no CPU fallback)"); return; }
         if (device < 0 || device >= n) { rc = ops_fail(HIPADJ_ERR_INVALID_ARG, "device %d out of range (%d visible)", device, n); return; }

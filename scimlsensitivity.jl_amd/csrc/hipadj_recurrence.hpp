@@ -187,7 +187,9 @@ template <class S, int V> struct Lds {
     uint32_t ticket;
 };
 
-template <class S> __device__ inline S through(S A, S H, uint32_t cut, S c) { return cut ? H : A * c + H; }
+// A state of exactly zero leaves H whatever A is: decays above one may have overflowed in A over the rows, and where one of them is not finite itself H says so already (it starts from
+// the same zero).
+template <class S> __device__ inline S through(S A, S H, uint32_t cut, S c) { return cut || c == S(0) ? H : A * c + H; }
 
 // The state at the start of position `k` of chain `c` (positions are in scan order; the adjoint counts tiles from the end), given the maps of its NW pieces in sh.A / sh.H / sh.cut
 // (piece order is scan order too).  `first`: the state at the chain's start.  Publishes what later tiles of the chain wait for.  Returns with all pieces' waves past a barrier.

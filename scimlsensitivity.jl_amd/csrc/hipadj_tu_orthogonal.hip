@@ -174,12 +174,13 @@ extern "C" int hipadj_orthogonalized_update_size(const hipadj_orthogonal* o, int
     return HIPADJ_OK;
 }
 
-extern "C" int hipadj_orthogonalized_update_dev(const hipadj_orthogonal* o, const void* grad, float* momentum, void* out, void* workspace, void* stream) {
+extern "C" int hipadj_orthogonalized_update_dev(const hipadj_orthogonal* o, const void* grad, float* momentum, void* out, void* workspace, int64_t workspace_bytes, void* stream) {
     const int rc = orth::check(o);
     if (rc != HIPADJ_OK) return rc;
     if (o->batch == 0 || o->rows == 0 || o->cols == 0) return HIPADJ_OK;
     const orth::Plan p = orth::plan_of(o, (char*)workspace);
-    if (!grad || !out || (p.bytes && (!workspace || (uintptr_t)workspace % 256))) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonalized_update_dev: grad, out and a 256-byte aligned workspace are required");
+    if (!grad || !out || (p.bytes && (!workspace || (uintptr_t)workspace % 256 || workspace_bytes < p.bytes)))
+        return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_orthogonalized_update_dev: grad, out and a 256-byte aligned workspace of %lld bytes are required", (long long)p.bytes);
     OpsDevice dev(o->device);
     if (dev.rc != HIPADJ_OK) return dev.rc;
     hipStream_t s = (hipStream_t)stream;

@@ -109,7 +109,7 @@ static bool fits(const void* p, const int64_t* st, int64_t bytes, int64_t V) {
     return !p || (((uintptr_t)p % (uintptr_t)(bytes * V)) == 0 && st[0] % V == 0 && st[1] % V == 0);
 }
 
-static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace, void* stream) {
+static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace, int64_t workspace_bytes, void* stream) {
     const int pair = pair_of(r->dtype, r->gate_dtype);
     const int64_t xb = size_of(r->dtype), gb = size_of(r->gate_dtype), VW = xb == 2 ? 2 : 1;
     const int64_t ntiles = tiles_of(r, adjoint);
@@ -135,7 +135,8 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
         return ops_launched("recurrence");
     }
     if (words) {
-        if (!workspace || (uintptr_t)workspace % 8) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: %lld rows need a workspace (hipadj_recurrence_sizes), 8-byte aligned", (long long)r->length);
+        if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < 8 * words)
+            return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: %lld rows need a workspace of %lld bytes (hipadj_recurrence_sizes), 8-byte aligned", (long long)r->length, (long long)(8 * words));
         uint64_t* w = (uint64_t*)workspace;
         const int64_t W = r->dtype == HIPADJ_F64 ? WPM<double> : WPM<float>;
         a.ticket = (uint32_t*)w; a.agg = w + 1; a.car = a.agg + (int64_t)a.nchains * a.ntiles * W * 64 * V;
@@ -157,25 +158,25 @@ extern "C" int hipadj_recurrence_sizes(const hipadj_recurrence* r, int64_t* chec
 }
 
 extern "C" int hipadj_recurrence_forward_dev(const hipadj_recurrence* r, const void* x, const void* gate, const void* h0, void* h, void* h_final, void* checkpoints,
-                                             void* workspace, void* stream) {
+                                             void* workspace, int64_t workspace_bytes, void* stream) {
     const int rc = rec::check(r);
     if (rc != HIPADJ_OK) return rc;
     if (r->channels == 0 || (r->nseq == 0 && r->batch == 0)) return HIPADJ_OK;
     if (!h_final || (r->length > 0 && (!x || !gate || !h))) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_recurrence_forward_dev: x, gate, h and h_final are required");
     rec::Args a{};
     a.x = x; a.gate = gate; a.h0 = h0; a.h = h; a.h_final = h_final; a.ckpt = checkpoints;
-    return rec::go(r, a, false, workspace, stream);
+    return rec::go(r, a, false, workspace, workspace_bytes, stream);
 }
 
 extern "C" int hipadj_recurrence_adjoint_dev(const hipadj_recurrence* r, const void* x, const void* gate, const void* h0, const void* checkpoints, const void* dh, const void* dh_final,
-                                             void* dx, void* dgate, void* dh0, void* workspace, void* stream) {
+                                             void* dx, void* dgate, void* dh0, void* workspace, int64_t workspace_bytes, void* stream) {
     const int rc = rec::check(r);
     if (rc != HIPADJ_OK) return rc;
     if (r->channels == 0 || (r->nseq == 0 && r->batch == 0)) return HIPADJ_OK;
     if (r->length > 0 && (!checkpoints || !x || !gate)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_recurrence_adjoint_dev: x, gate and the forward pass's checkpoints are required");
     rec::Args a{};
     a.x = x; a.gate = gate; a.h0 = h0; a.ckpt = const_cast<void*>(checkpoints); a.dh = dh; a.dh_final = dh_final; a.dx = dx; a.dgate = dgate; a.dh0 = dh0;
-    return rec::go(r, a, true, workspace, stream);
+    return rec::go(r, a, true, workspace, workspace_bytes, stream);
 }
 
 extern "C" int hipadj_recurrence_step_dev(int32_t device, int32_t dtype, int32_t gate_dtype, int32_t gate_form, int32_t coupled, int64_t batch, int64_t channels, const void* x,

@@ -114,7 +114,7 @@ def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
     sol.h, sol.h_final = h, torch.empty((rows, channels), dtype=wide, device=x.device)
     sol._checkpoints = torch.empty(ck.value, dtype=torch.uint8, device=x.device) if adjoint else None
     work = torch.empty(ws.value, dtype=torch.uint8, device=x.device) if ws.value else None
-    _check(L.hipadj_recurrence_forward_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(h0), _ptr(h), _ptr(sol.h_final), _ptr(sol._checkpoints), _ptr(work), _stream(torch, x.device)))
+    _check(L.hipadj_recurrence_forward_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(h0), _ptr(h), _ptr(sol.h_final), _ptr(sol._checkpoints), _ptr(work), ws.value, _stream(torch, x.device)))
     sol.x, sol.gate, sol.h0, sol.offsets, sol.form, sol.coupled = x, gate, h0, offsets, form, bool(coupled)
     sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape = r, ws.value, wide, (rows, channels)
     return sol
@@ -142,7 +142,7 @@ def recurrence_adjoint(sol, dh=None, dh_final=None, *, need=(True, True, True)):
         r.dgate_stride[:] = _strides(dgate, packed)
     work = torch.empty(sol._workspace_bytes, dtype=torch.uint8, device=x.device) if sol._workspace_bytes else None
     _check(_lib.load().hipadj_recurrence_adjoint_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(sol.h0), _ptr(sol._checkpoints), _ptr(dh), _ptr(dh_final), _ptr(dx), _ptr(dgate), _ptr(dh0),
-                                                     _ptr(work), _stream(torch, x.device)))
+                                                     _ptr(work), sol._workspace_bytes, _stream(torch, x.device)))
     return dx, dgate, dh0
 
 
@@ -269,5 +269,5 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     ws = C.c_int64()
     _check(L.hipadj_orthogonalized_update_size(C.byref(q), C.byref(ws)))
     work = torch.empty(ws.value, dtype=torch.uint8, device=grad.device) if ws.value else None
-    _check(L.hipadj_orthogonalized_update_dev(C.byref(q), _ptr(g), _ptr(m), _ptr(o), _ptr(work), _stream(torch, grad.device)))
+    _check(L.hipadj_orthogonalized_update_dev(C.byref(q), _ptr(g), _ptr(m), _ptr(o), _ptr(work), ws.value, _stream(torch, grad.device)))
     return given_out if given_out is not None else out

@@ -149,6 +149,16 @@ def test_nan_and_infinite_rows_go_on_in_their_sequence(sa, torch):
     compare(sa, torch, q, "sigmoid", True, "float32")
 
 
+def test_growing_decays_on_states_of_zero(sa, torch):
+    """Decays of two overflow as a product over 128 rows; a state that is still exactly zero stays zero, forward and in the adjoint, and what starts later grows as it should."""
+    q = inputs(torch, 21, (1, 700, 6), 1, "decay", "float32")
+    q["gate"].fill_(2.0); q["x"].zero_(); q["h0"].zero_(); q["dh"].zero_(); q["dhf"].zero_()
+    q["x"][0, 690, 1] = 3.0; q["dh"][0, 12, 2] = 1.5
+    sol, (dx, dg, d0) = compare(sa, torch, q, "decay", False, "float32")
+    assert float(sol.h[0, 699, 1]) == 3.0 * 2.0 ** 9 and float(dx[0, 0, 2]) == 1.5 * 2.0 ** 12 and float(d0[0, 2]) == 1.5 * 2.0 ** 13
+    assert int(torch.count_nonzero(sol.h)) == 10 and int(torch.count_nonzero(dx)) == 13
+
+
 def test_strides_of_fused_projections_and_broadcast_gates(sa, torch):
     q = inputs(torch, 11, (2, 150, 64), 2, "log", "bfloat16")
     both = torch.empty(2, 150, 128, dtype=torch.bfloat16, device="cuda")

@@ -41,8 +41,8 @@ def test_recurrence_refusals(lib, kw, status, text):
     _lib, L = lib
     r = recurrence(_lib, **kw)
     assert L.hipadj_recurrence_sizes(C.byref(r), None, None) == status and text in L.hipadj_last_error(None).decode()
-    assert L.hipadj_recurrence_forward_dev(C.byref(r), *[256] * 8) == status
-    assert L.hipadj_recurrence_adjoint_dev(C.byref(r), *[256] * 11) == status
+    assert L.hipadj_recurrence_forward_dev(C.byref(r), *[256] * 9) == status
+    assert L.hipadj_recurrence_adjoint_dev(C.byref(r), *[256] * 12) == status
 
 
 def test_recurrence_arguments_and_sizes(lib):
@@ -53,9 +53,9 @@ def test_recurrence_arguments_and_sizes(lib):
     assert ck.value == 2 * 5 * 70 * 4 and ws.value > 0                       # a checkpoint every 64 rows
     short = recurrence(_lib, length=64)
     assert L.hipadj_recurrence_sizes(C.byref(short), None, C.byref(ws)) == 0 and ws.value == 0
-    assert L.hipadj_recurrence_forward_dev(C.byref(r), None, 256, None, 256, 256, None, 256, None) == -1
-    assert L.hipadj_recurrence_adjoint_dev(C.byref(r), 256, 256, None, None, None, None, 256, 256, 256, 256, None) == -1 and b"checkpoints" in L.hipadj_last_error(None)
-    assert L.hipadj_recurrence_forward_dev(C.byref(recurrence(_lib, batch=0)), *[None] * 8) == 0
+    assert L.hipadj_recurrence_forward_dev(C.byref(r), None, 256, None, 256, 256, None, 256, ws.value, None) == -1
+    assert L.hipadj_recurrence_adjoint_dev(C.byref(r), 256, 256, None, None, None, None, 256, 256, 256, 256, 0, None) == -1 and b"checkpoints" in L.hipadj_last_error(None)
+    assert L.hipadj_recurrence_forward_dev(C.byref(recurrence(_lib, batch=0)), *[None] * 7, 0, None) == 0
     step = lambda **k: L.hipadj_recurrence_step_dev(*{**dict(device=0, dtype=1, gate_dtype=1, gate=1, coupled=0, batch=2, channels=4, x=256, xs=4, g=256, gs=4, st=256, ss=4, n=2,     # noqa: E731
                                                               slots=None, bits=32, h=256, hs=4, stream=None), **k}.values())
     assert step(n=1) == -1 and step(gate=5) == -1 and step(dtype=2, gate_dtype=0) == -6 and step(x=None) == -1 and step(slots=256, bits=8) == -1 and step(batch=-1) == -1
@@ -73,16 +73,17 @@ def test_orthogonal_refusals(lib, kw, status, text):
     assert L.hipadj_orthogonalized_update_size(C.byref(o), C.byref(ws)) == status
     if status:
         assert text in L.hipadj_last_error(None).decode()
-        assert L.hipadj_orthogonalized_update_dev(C.byref(o), *[256] * 4, None) == status
+        assert L.hipadj_orthogonalized_update_dev(C.byref(o), *[256] * 4, 0, None) == status
 
 
 def test_orthogonal_arguments(lib):
     _lib, L = lib
     o = orthogonal(_lib)
-    assert L.hipadj_orthogonalized_update_dev(C.byref(o), None, None, 256, 256, None) == -1
+    assert L.hipadj_orthogonalized_update_dev(C.byref(o), None, None, 256, 256, 0, None) == -1
     large = orthogonal(_lib, rows=400)
-    assert L.hipadj_orthogonalized_update_dev(C.byref(large), 256, None, 256, 128, None) == -1 and b"aligned" in L.hipadj_last_error(None)
-    assert L.hipadj_orthogonalized_update_dev(C.byref(orthogonal(_lib, rows=0)), None, None, None, None, None) == 0
+    assert L.hipadj_orthogonalized_update_dev(C.byref(large), 256, None, 256, 128, 1 << 40, None) == -1 and b"aligned" in L.hipadj_last_error(None)
+    assert L.hipadj_orthogonalized_update_dev(C.byref(large), 256, None, 256, 256, 1000, None) == -1
+    assert L.hipadj_orthogonalized_update_dev(C.byref(orthogonal(_lib, rows=0)), None, None, None, None, 0, None) == 0
 
 
 def test_no_cpu_fallback(sa):
