@@ -149,6 +149,17 @@ def test_nan_and_infinite_rows_go_on_in_their_sequence(sa, torch):
     compare(sa, torch, q, "sigmoid", True, "float32")
 
 
+@pytest.mark.parametrize("form", ["decay", "log", "sigmoid"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_gradient_of_a_start_behind_a_strong_decay(sa, torch, form, packed):
+    """dh0 = a_1 G_1 leaves in 32 bits also for 16-bit data: exact where a_1 is tiny."""
+    q = inputs(torch, 22, (1, 40, 34), 1, form, "bfloat16")
+    q["gate"][0, 0] = {"decay": 2e-4, "log": -9.0, "sigmoid": -9.0}[form]
+    if packed:
+        q = {k: v[0] if v.dim() == 3 else v for k, v in q.items()}
+    compare(sa, torch, q, form, True, "bfloat16", offsets=[0, 40] if packed else None)
+
+
 def test_growing_decays_on_states_of_zero(sa, torch):
     """Decays of two overflow as a product over 128 rows; a state that is still exactly zero stays zero, forward and in the adjoint, and what starts later grows as it should."""
     q = inputs(torch, 21, (1, 700, 6), 1, "decay", "float32")
