@@ -61,12 +61,15 @@ template <class T> __device__ inline float moved(const Io<T>& io, int64_t b, int
     return io.nesterov ? g + io.beta * m : m;
 }
 
-__device__ inline double block_sum(double v) {       // 256 threads, fixed order
-    __shared__ double s[4];
+template <int WAVES> __device__ inline double block_sum(double v) {       // fixed order
+    __shared__ double s[WAVES];
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
     if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (s[0] + s[1]) + (s[2] + s[3]);
+    double t = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) t += s[w];
+    return t;
 }
 
 // Momentum and the partial sums of |u|^2.  A workgroup takes stretches of NORM_SPAN neighbouring elements (host side: matrices without gaps count as one row), 8 a thread with one
@@ -101,29 +104,31 @@ template <class T> __global__ void __launch_bounds__(256) k_norm(const Io<T> io,
             for (int64_t c = c0 + threadIdx.x; c < cols && c < c0 + NORM_SPAN; c += 256) { const float u = moved(io, b, r, c, true); s += (double)u * (double)u; }
         }
     }
-    s = block_sum(s);
+    s = block_sum<4>(s);
     if (threadIdx.x == 0) partial[b * gridDim.x + blockIdx.x] = s;
 }
 
 template <bool SPLIT> __device__ inline void terms(float v, f16& hi, f16& lo) { hi = (f16)v; if constexpr (SPLIT) lo = (f16)(v - (float)hi); }
 
-// X = u / (|u| + 1e-7) in both orders, padding included.  A workgroup takes a 64 x 64 piece through LDS.
-template <class T, bool SPLIT> __global__ void __launch_bounds__(256) k_start(const Io<T> io, const Mat q) {
+// X = u / (|u| + 1e-7) in both orders, padding included.  A workgroup takes a 64 x 64 piece through LDS: reads 2 or 4 bytes of gradient and momentum an element, writes 2 + 2 (two-term: 4 + 4)
+// and the 4 of the FP32 copy; memory-bound where there are many pieces (4096 x 4096 bf16 with momentum, 14 B an element: 50 us, 4.7 TB/s), one piece's latency where there are few.  Hence
+// four waves, or 16 up to four pieces a CU: 48 pieces of 333 x 500 7.6 us (four waves: 12.2), 1024 pieces of 16 x 256 x 1024 18.1 (19.5), but 4096 pieces 60.7 (49.6).
+template <class T, bool SPLIT, int WAVES> __global__ void __launch_bounds__(WAVES * 64) k_start(const Io<T> io, const Mat q) {
     __shared__ float tile[64][65];
     const int64_t b = blockIdx.z, i0 = (int64_t)blockIdx.y * 64, j0 = (int64_t)blockIdx.x * 64;      // rows and columns of X
     double s = 0;
-    for (int i = threadIdx.x; i < q.nblocks; i += 256) s += q.partial[b * q.nblocks + i];
-    s = block_sum(s);
+    for (int i = threadIdx.x; i < q.nblocks; i += WAVES * 64) s += q.partial[b * q.nblocks + i];
+    s = block_sum<WAVES>(s);
     const double inv = (double)SX / (sqrt(s) + 1e-7);
     const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int r = w; r < 64; r += 4) {                         // lanes run along the caller's rows
+    for (int r = w; r < 64; r += WAVES) {                     // lanes run along the caller's rows
         const int64_t i = q.flip ? i0 + l : i0 + r, j = q.flip ? j0 + r : j0 + l;
         float v = 0.f;
         if (i < q.m && j < q.n) v = (float)((double)(q.flip ? moved(io, b, j, i, false) : moved(io, b, i, j, false)) * inv);
         tile[q.flip ? l : r][q.flip ? r : l] = v;
     }
     __syncthreads();
-    for (int r = w; r < 64; r += 4) {
+    for (int r = w; r < 64; r += WAVES) {
         f16 hi, lo;
         terms<SPLIT>(tile[r][l], hi, lo);
         const int64_t at = (b * q.mp + i0 + r) * q.np + j0 + l;

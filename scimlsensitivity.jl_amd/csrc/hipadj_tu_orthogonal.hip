@@ -88,7 +88,9 @@ template <class T, bool SPLIT> static void iterate(const hipadj_orthogonal* o, c
     auto aligned = [&](const void* p, int64_t sb, int64_t sr, int64_t per) { return (uintptr_t)p % 16 == 0 && (q.batch == 1 || sb % per == 0) && (rows == 1 || sr % per == 0); };
     const bool vec = cols % 8 == 0 && aligned(io.grad, io.g_b, io.g_r, 16 / sizeof(T)) && (!io.mom || aligned(io.mom, io.m_b, io.m_r, 4));
     k_norm<T><<<dim3((uint32_t)q.nblocks, (uint32_t)q.batch), dim3(256), 0, s>>>(io, rows, cols, vec, q.partial);
-    k_start<T, SPLIT><<<dim3((uint32_t)(q.np / 64), (uint32_t)(q.mp / 64), (uint32_t)q.batch), dim3(256), 0, s>>>(io, q);
+    const dim3 pieces((uint32_t)(q.np / 64), (uint32_t)(q.mp / 64), (uint32_t)q.batch);
+    if (q.np / 64 * (q.mp / 64) * q.batch <= 1024) k_start<T, SPLIT, 16><<<pieces, dim3(1024), 0, s>>>(io, q);
+    else k_start<T, SPLIT, 4><<<pieces, dim3(256), 0, s>>>(io, q);
     const int64_t smm = q.mp * q.mp, smn = q.mp * q.np;
     auto rounded = [&](int step) { return !SPLIT && step >= o->steps - 2; };
     for (int step = 0; step < o->steps; ++step) {
