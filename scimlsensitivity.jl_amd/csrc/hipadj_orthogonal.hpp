@@ -73,7 +73,7 @@ template <int WAVES> __device__ inline double block_sum(double v) {       // fix
 }
 
 // Momentum and the partial sums of |u|^2.  A workgroup takes stretches of NORM_SPAN neighbouring elements (host side: matrices without gaps count as one row), 8 a thread with one
-// request where rows start on 16 bytes.  Reads 2 or 4 + 4 bytes an element, writes 4: memory-bound.
+// request where rows start on 16 bytes.  Reads 2 or 4 + 4 bytes an element, writes 4: memory-bound (4096 x 4096 bf16 with momentum: 31 us, 5.4 TB/s, part of it from the last-level cache).
 constexpr int NORM_SPAN = 2048;
 template <class T> __global__ void __launch_bounds__(256) k_norm(const Io<T> io, int64_t rows, int64_t cols, bool vec, double* partial) {
     const int64_t b = blockIdx.y;
@@ -153,6 +153,10 @@ template <class T, bool SPLIT, int WAVES> __global__ void __launch_bounds__(WAVE
 //
 // In a stage the factors of its second half are read while the first half is multiplied, and those of the next stage's first half while the second is; the one barrier stands between the
 // halves: behind it the next stage has arrived in every wave's part, and no wave still reads this stage's buffer, which stage s + 4 is requested into.
+//
+// Bound: the matrix cores, at the clock that the board's power leaves (1.95 GHz while they are busy).  4096 x 4096, one term: X X' and the polynomial of A, half their tiles each, 92 and 96 us
+// (750 and 715 TFLOP/s of the half), B X with X out in three forms 147-163 us (840-930).  Small sides: a launch of 4-9 us each, most of it the latency of the first stages and of the
+// epilogue (two groups of four waves that share a tile and halve K were 10 % slower at every size).
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
 
 struct Product {
@@ -412,7 +416,7 @@ __global__ void __launch_bounds__(256, BT == 64 || (BT == 128 && SLOTS == 1) ? 2
 }
 
 // ---- small matrices ---------------------------------------------------------------------------------------------------------------------------------------------------
-// Both sides at most 128: one workgroup does a matrix in one launch (17 otherwise, each a few microseconds of latency).  X, A and B live in LDS as two F16 terms and 32 x 32 pieces of X
+// Both sides at most 128: one workgroup does a matrix in one launch (17 otherwise: 48.6 us against 205 at 128 x 128).  X, A and B live in LDS as two F16 terms and 32 x 32 pieces of X
 // stay in the F32 registers of the waves that own them.  X is needed by rows for X X' and by columns for B X, never at once, and A, B never next to X by rows: two regions, 128 KB at
 // a side of 128.  Symmetric matrices are stored transposed, which is their own order, four neighbours at a time.
 template <class T, int S> __global__ void __launch_bounds__((S / 32) * (S / 32) * 64) k_small(const Io<T> io, const int64_t m, const int64_t n, const bool flip, const int steps, const Coefficients co) {

@@ -92,6 +92,8 @@ static int64_t words_of(const hipadj_recurrence* r, int64_t ntiles, int V) {
     return 1 + chains * CW * ((wide ? WPM<double> : WPM<float>) * ntiles + (wide ? WPV<double> : WPV<float>) * ((ntiles + GS - 1) / GS));
 }
 
+constexpr int64_t MOST_THREADS = (int64_t(1) << 32) - 1;      // of a launch, in a dimension
+
 static int check(const hipadj_recurrence* r) {
     if (!r || r->struct_size != sizeof(hipadj_recurrence)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_recurrence.struct_size does not match this library");
     if (pair_of(r->dtype, r->gate_dtype) < 0) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence: x is F64, F32, BF16 or F16 and the gate of x's type, or F32 next to BF16 / F16");
@@ -122,6 +124,8 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
     a.dh_sb = r->dh_stride[0]; a.dh_st = r->dh_stride[1]; a.dx_sb = r->dx_stride[0]; a.dx_st = r->dx_stride[1]; a.dg_sb = r->dgate_stride[0]; a.dg_st = r->dgate_stride[1];
     a.L = r->length; a.D = r->channels; a.nseq = r->nseq; a.offsets = r->offsets; a.offsets64 = r->offsets_bits == 64;
     a.ntiles = (int)ntiles; a.nckpt = (int)tiles_of(r, true); a.ncg = (int)((r->channels + 64 * V - 1) / (64 * V)); a.nchains = (int)(r->batch * a.ncg); a.GS = group_of(a.nchains);
+    if ((int64_t)a.ntiles * a.nchains > MOST_THREADS / NT)
+        return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence: %lld tiles, a launch has at most %lld workgroups: fewer batch rows at a time", (long long)a.ntiles * a.nchains, (long long)(MOST_THREADS / NT));
     const int64_t words = words_of(r, ntiles, V);
     OpsDevice dev(r->device);
     if (dev.rc != HIPADJ_OK) return dev.rc;
@@ -190,10 +194,11 @@ extern "C" int hipadj_recurrence_step_dev(int32_t device, int32_t dtype, int32_t
     if (!x || !gate || !h || (!state && nslots > 0)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "hipadj_recurrence_step_dev: x, gate, state and h are required");
     if (slots && slots_bits != 32 && slots_bits != 64) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence step: slots_bits must be 32 or 64");
     if (!slots && nslots < batch) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence step: %lld rows without slots need as many states, got %lld", (long long)batch, (long long)nslots);
-    if (batch > ((int64_t(1) << 31) - 1) / ((channels + rec::NS - 1) / rec::NS)) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence step: more than 2^31 - 1 workgroups");
     const int64_t xb = rec::size_of(dtype), gb = rec::size_of(gate_dtype), sb = dtype == HIPADJ_F64 ? 8 : 4, VW = xb == 2 ? 2 : 1;
     auto fits = [&](const void* p, int64_t st, int64_t bytes) { return (uintptr_t)p % (uintptr_t)(bytes * VW) == 0 && st % VW == 0; };
     const bool wide = VW == 1 || (channels % VW == 0 && fits(x, x_stride, xb) && fits(gate, gate_stride, gb) && fits(h, h_stride, xb) && fits(state, state_stride, sb));
+    if (batch > rec::MOST_THREADS / rec::NS / ((channels + rec::NS * (wide ? VW : 1) - 1) / (rec::NS * (wide ? VW : 1))))
+        return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence step: %lld rows of %lld channels, a launch has at most %lld workgroups", (long long)batch, (long long)channels, (long long)(rec::MOST_THREADS / rec::NS));
     rec::StepArgs a{x, gate, slots, state, h, x_stride, gate_stride, state_stride, h_stride, batch, channels, nslots, slots_bits == 64};
     OpsDevice dev(device);
     if (dev.rc != HIPADJ_OK) return dev.rc;

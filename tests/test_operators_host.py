@@ -62,6 +62,20 @@ def test_recurrence_arguments_and_sizes(lib):
     assert step(batch=0) == 0
 
 
+def test_recurrence_launch_limits(lib):
+    """A launch has 2^32 - 1 threads: more tiles of 512 or more step rows of 256 are refused by name, the largest that fit get as far as the device."""
+    _lib, L = lib
+    most = (2 ** 32 - 1) // 512
+    r = lambda b: C.byref(recurrence(_lib, batch=b, length=1, channels=64, device=1 << 20))                                                     # noqa: E731
+    for b, refused in ((most + 1, True), (most, False)):
+        for status in (L.hipadj_recurrence_forward_dev(r(b), *[256] * 7, 0, None), L.hipadj_recurrence_adjoint_dev(r(b), *[256] * 10, 0, None)):
+            assert (status == -6) == refused and status != 0 and (b"at a time" in L.hipadj_last_error(None)) == refused
+    most = (2 ** 32 - 1) // 256
+    for b, refused in ((most + 1, True), (most, False), (most // 2 + 1, False)):
+        status = L.hipadj_recurrence_step_dev(1 << 20, 1, 1, 1, 0, b, 4, 256, 4, 256, 4, 256, 4, b, None, 32, 256, 4, None)
+        assert (status == -6) == refused and status != 0 and (b"at most" in L.hipadj_last_error(None)) == refused
+
+
 @pytest.mark.parametrize("kw,status,text", [
     (dict(struct_size=4), -1, "struct_size"), (dict(dtype=0), -6, "F32, BF16 or F16"), (dict(rows=-1), -1, "negative"), (dict(steps=0), -1, "steps"), (dict(steps=65), -1, "steps"),
     (dict(beta=float("nan")), -1, "finite"), (dict(rows=70000, cols=70000), -6, "at most"), (dict(batch=65536), -6, "at most"), (dict(coefficients=(33.0, 0.0, 0.0)), -1, "within"),
