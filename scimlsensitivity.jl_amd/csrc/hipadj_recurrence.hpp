@@ -21,10 +21,10 @@
 // registers — the bytes of reading h back are those of reading x, and the states are the unrounded ones.
 // Bound: memory, 3 streams forward and 5 in the adjoint, where the axes are long and many; the exchanges along the chain where there are few.  Measured on an MI355X (a copy: 5.10 TB/s), the
 // launch of k_zero (2-6 us) not counted:
-//   forward  1 x 65536 x 2048 BF16, exp gate            194 us, 4.16 TB/s        8 x 4096 x 2048 BF16, coupled sigmoid, with checkpoints  103 us, 3.95 TB/s
-//            37 packed sequences, 16381 x 1024 F16       45 us, 2.2 TB/s         2 x 2047 x 777 F32                                        16 us, 2.5 TB/s
+//   forward  1 x 65536 x 2048 BF16, exp gate            194 us, 4.16 TB/s        8 x 4096 x 2048 BF16, coupled sigmoid, with checkpoints   98 us, 4.15 TB/s
+//            37 packed sequences, 16381 x 1024 F16       36 us, 2.8 TB/s         2 x 2047 x 777 F32                                        16 us, 2.5 TB/s
 //            1 x 512 x 2048 BF16                        8.8 us: four tiles a chain, latency
-//   adjoint  8 x 4096 x 2048 BF16, coupled sigmoid      170 us, 4.0 TB/s         2 x 2047 x 777 F32                                        26 us, 2.4 TB/s
+//   adjoint  8 x 4096 x 2048 BF16, coupled sigmoid      164 us, 4.1 TB/s         2 x 2047 x 777 F32                                        26 us, 2.4 TB/s
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -36,6 +36,7 @@ constexpr int TSF = 16;           // rows of a piece, forward: (a, b) of 16 x V 
 constexpr int TSA = 8;            // rows of a piece, adjoint: five values a cell, so half as many (16 spilled 47 ... 101 registers and left one workgroup a CU)
 constexpr int TTF = NW * TSF, TTA = NW * TSA;                 // rows of a tile; a checkpoint every TTA rows
 constexpr int NT = NW * 64;
+constexpr int MOST_GS = 32;       // tiles of a group: a multiple of NW up to this
 
 typedef __bf16 bf16;
 typedef _Float16 f16;
@@ -128,13 +129,14 @@ __device__ inline void publish_map(uint64_t* w, int64_t, float A, float H, uint3
     put(w, (uint64_t(__float_as_uint(H)) << 32) | (cut ? 1u : a));
 }
 __device__ inline void publish_map(uint64_t* w, int64_t cw, double A, double H, uint32_t cut) { publish(w, cw, A, cut ? TAG_CUT : TAG_VALUE); publish(w + 2 * cw, cw, H, TAG_VALUE); }
-__device__ inline uint32_t await_map(const uint64_t* w, int64_t, float& A, float& H) {
-    uint64_t q;
-    while (!((q = get(w)) & 1u)) __builtin_amdgcn_s_sleep(1);
+// `seen`: the first look at the word, taken earlier so that several are on their way together (64 bits: none)
+__device__ inline uint32_t await_map(const uint64_t* w, int64_t, uint64_t seen, float& A, float& H) {
+    uint64_t q = seen;
+    while (!(q & 1u)) { __builtin_amdgcn_s_sleep(1); q = get(w); }
     A = __uint_as_float((uint32_t)q); H = __uint_as_float((uint32_t)(q >> 32));
     return (uint32_t)q == 1u;
 }
-__device__ inline uint32_t await_map(const uint64_t* w, int64_t cw, double& A, double& H) {
+__device__ inline uint32_t await_map(const uint64_t* w, int64_t cw, uint64_t, double& A, double& H) {
     const uint32_t q = await_value(w, cw, A);
     await_value(w + 2 * cw, cw, H);
     return q == TAG_CUT;
@@ -142,17 +144,23 @@ __device__ inline uint32_t await_map(const uint64_t* w, int64_t cw, double& A, d
 
 // ---- packed sequences ---------------------------------------------------------------------------------------------------------------------------------------------
 
-__device__ inline int64_t offset_at(const Args& p, int64_t i) { return p.offsets64 ? ((const int64_t*)p.offsets)[i] : (int64_t)((const int32_t*)p.offsets)[i]; }
+struct Offset { uint32_t lo, hi; };                           // as it arrives (32 bits: twice the same word), so that nothing waits where it is requested
+__device__ inline Offset request_offset(const Args& p, int64_t i) {
+    const uint32_t* w = (const uint32_t*)p.offsets + (i << p.offsets64);
+    return {w[0], w[p.offsets64]};
+}
+__device__ inline int64_t value_of(const Args& p, Offset o) { return p.offsets64 ? (int64_t)((uint64_t)o.hi << 32 | o.lo) : (int64_t)(int32_t)o.lo; }
+__device__ inline int64_t offset_at(const Args& p, int64_t i) { return value_of(p, request_offset(p, i)); }
 
-// the first sequence that ends behind row t (nseq: none), found by a 64-ary search over the ends; offsets that do not ascend give some number in [0, nseq]
-__device__ inline int64_t seq_behind(const Args& p, int64_t t) {
-    int64_t lo = 0, n = p.nseq;                               // the answer is in [lo, lo + n]
+// The first sequence that ends behind row t (nseq: none) is among lo ... lo + 63: a 64-ary search over the ends.  Offsets that do not ascend give some number in [0, nseq].
+__device__ inline int64_t narrow(const Args& p, int64_t t) {
+    int64_t lo = 0, n = p.nseq;                               // it is in [lo, lo + n]
     const int lane = threadIdx.x & 63;
-    while (n > 0) {
+    while (n > 63) {
         const int64_t step = (n + 63) / 64;
-        const int64_t i = lo + (int64_t)lane * step + step - 1;                     // last of this lane's stretch
-        const bool in = (int64_t)lane * step < n;
-        const int64_t last = i < lo + n ? i : lo + n - 1;
+        const int64_t i = lo + lane * step;
+        const bool in = lane * step < n;
+        const int64_t last = i + step - 1 < lo + n ? i + step - 1 : lo + n - 1;
         const bool before = in && offset_at(p, last + 1) <= t;                      // the whole stretch ends at t or earlier
         const int k = __popcll(__ballot(before));
         const int64_t at = (int64_t)k * step;
@@ -162,24 +170,55 @@ __device__ inline int64_t seq_behind(const Args& p, int64_t t) {
     }
     return lo;
 }
+__device__ inline int64_t of_lane(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)v, lane) | (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32);
+}
 
 struct Marks { uint32_t start, end, out; };                   // bits of a piece's rows: first of a sequence, last of one, of none
-template <int TS> __device__ inline Marks marks_of(const Args& p, int64_t t0) {
+// The bounds of 64 neighbouring sequences, one a lane, among them the first that ends behind row t: one exchange with memory for up to 63 sequences.  Requested BEFORE the rows: requests
+// return in order, and behind the rows' they would keep the arithmetic waiting for the last row (1 x 16384 x 1024 F16, one sequence: 44 us instead of 40).
+struct Window { int64_t lo; Offset start, end; bool in; };
+__device__ inline Window window_of(const Args& p, int64_t t) {
+    Window w{};
+    w.lo = narrow(p, t);
+    const int64_t s = w.lo + (threadIdx.x & 63);
+    w.in = s < p.nseq;
+    const int64_t i = w.in ? s : p.nseq - 1;
+    w.start = request_offset(p, i); w.end = request_offset(p, i + 1);
+    return w;
+}
+// seq[i]: the sequence that row i, first or last of it, belongs to; in LDS, where the few rows that need it find it without a search (a search at each of those places made the adjoint of 37
+// sequences of 16384 x 1024 F16 take 78-96 us instead of 64)
+template <int TS> __device__ inline Marks marks_of(const Args& p, int64_t t0, Window w, int64_t (&seq)[TS]) {
     Marks m{0, 0, (1u << TS) - 1};
-    int64_t pos = t0;
+    int64_t pos = t0, start = value_of(p, w.start), end = value_of(p, w.end);
     while (pos < t0 + TS && pos < p.L) {                      // pos advances in every turn, whatever the offsets hold
-        const int64_t s = seq_behind(p, pos);
-        if (s >= p.nseq) break;
-        const int64_t st = offset_at(p, s), en = offset_at(p, s + 1);
+        int k = __popcll(__ballot(w.in && end <= pos));
+        if (k == 64) {
+            w = window_of(p, pos);
+            start = value_of(p, w.start); end = value_of(p, w.end);
+            k = __popcll(__ballot(w.in && end <= pos));
+        }
+        if (k == 64 || w.lo + k >= p.nseq) break;
+        const int64_t st = of_lane(start, k), en = of_lane(end, k);
         const int64_t from = st > pos ? st : pos, to = en < t0 + TS ? en : t0 + TS;
-        for (int64_t t = from; t < to; ++t) m.out &= ~(1u << (int)(t - t0));
-        if (st >= t0 && st < to) m.start |= 1u << (int)(st - t0);
-        if (en - 1 >= from && en - 1 < t0 + TS) m.end |= 1u << (int)(en - 1 - t0);
+        if (from < to) m.out &= ~((1u << (int)(to - t0)) - (1u << (int)(from - t0)));      // bits from - t0 ... to - t0 - 1; both at most TS <= 16
+        if (st >= t0 && st < to) { m.start |= 1u << (int)(st - t0); seq[(int)(st - t0)] = w.lo + k; }
+        if (en - 1 >= from && en - 1 < t0 + TS) { m.end |= 1u << (int)(en - 1 - t0); seq[(int)(en - 1 - t0)] = w.lo + k; }
         pos = en > pos ? en : pos + 1;
     }
-    for (int i = 0; i < TS; ++i) if (t0 + i >= p.L) { m.out |= 1u << i; m.start &= ~(1u << i); m.end &= ~(1u << i); }
+    const int inside = p.L - t0 >= TS ? TS : p.L > t0 ? (int)(p.L - t0) : 0;
+    const uint32_t rows = (1u << inside) - 1;                 // rows behind the end belong to none
+    m.out |= ((1u << TS) - 1) & ~rows; m.start &= rows; m.end &= rows;
     m.start = __builtin_amdgcn_readfirstlane(m.start); m.end = __builtin_amdgcn_readfirstlane(m.end); m.out = __builtin_amdgcn_readfirstlane(m.out);
     return m;
+}
+__device__ inline int64_t uniform(int64_t v) { return of_lane(v, 0); }
+// Packed rows in two forms: most pieces have no mark and run as those of one long sequence.
+template <bool B> struct Flag { static constexpr bool value = B; };
+template <bool PACKED, class F> __device__ inline void by_marks(const Marks& m, F f) {
+    if constexpr (PACKED) { if (m.start | m.end | m.out) f(Flag<true>{}); else f(Flag<false>{}); }
+    else f(Flag<false>{});
 }
 
 // ---- the scan over the tiles of a chain -----------------------------------------------------------------------------------------------------------------------------
@@ -221,28 +260,47 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             for (int v = 0; v < V; ++v) publish_map(dst + v, CW, A[v], H[v], cut);
         }
     }
-    // the maps of the group's earlier tiles, NW at a time, one a wave; composed to (B, G)
+    // the maps of the group's earlier tiles: a wave takes GS / NW neighbouring ones, all requested before the first is waited for, and composes them; the waves' maps are composed to (B, G)
+    const int per = p.GS / NW, j0 = wave * per;
+    if (j0 < before) {
+        const uint64_t* src = p.agg + (c * p.ntiles + base + j0) * WM * CW + ch;
+        uint64_t seen[MOST_GS / NW][V];
+#pragma unroll
+        for (int m = 0; m < MOST_GS / NW; ++m)
+#pragma unroll
+            for (int v = 0; v < V; ++v) seen[m][v] = sizeof(S) == 4 && m < per && j0 + m < before ? get(src + m * WM * CW + v) : 0;
+        S a[V], h[V];
+        uint32_t q = 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) { a[v] = S(1); h[v] = S(0); }
+#pragma unroll
+        for (int m = 0; m < MOST_GS / NW; ++m)
+            if (m < per && j0 + m < before) {
+                uint32_t qm = 0;
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    S am, hm;
+                    qm = await_map(src + m * WM * CW + v, CW, seen[m][v], am, hm);
+                    h[v] = through(am, hm, qm, h[v]); a[v] *= am;
+                }
+                q |= qm;
+            }
+#pragma unroll
+        for (int v = 0; v < V; ++v) { sh.pA[wave][ch + v] = a[v]; sh.pH[wave][ch + v] = h[v]; }
+        if (lane == 0) sh.pcut[wave] = q;
+    }
     S B[V], G[V];
     uint32_t gcut = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) { B[v] = S(1); G[v] = S(0); }
-    for (int j0 = 0; j0 < before; j0 += NW) {
-        const int j = j0 + wave;
-        if (j < before) {
-            const uint64_t* src = p.agg + (c * p.ntiles + base + j) * WM * CW + ch;
-            uint32_t q = 0;
-#pragma unroll
-            for (int v = 0; v < V; ++v) q = await_map(src + v, CW, sh.pA[wave][ch + v], sh.pH[wave][ch + v]);
-            if (lane == 0) sh.pcut[wave] = q;
-        }
+    if (before > 0) {
         __syncthreads();
-        for (int i = 0; i < NW && j0 + i < before; ++i) {
+        for (int i = 0; i * per < before; ++i) {
             const uint32_t q = sh.pcut[i];
             gcut |= q;
 #pragma unroll
             for (int v = 0; v < V; ++v) { G[v] = through(sh.pA[i][ch + v], sh.pH[i][ch + v], q, G[v]); B[v] *= sh.pA[i][ch + v]; }
         }
-        __syncthreads();
     }
     // the state at the group's start: wave 0 waits for it and, in the group's last tile, has the next group's on its way two operations later
     if (g > 0) {
@@ -324,6 +382,7 @@ template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED
 __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Args p) {
     __shared__ Lds<S, V> sh;
     constexpr int TS = TSF;
+    __shared__ int64_t seqs[PACKED ? NW : 1][TS];
     constexpr bool FAST = sizeof(T) == 2 && sizeof(TG) == 2;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t tile = take(p, &sh.ticket);
@@ -333,10 +392,12 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
     const bool on = lane * V < q.channels;
     const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T);     // lanes past the last channel read the first one and write nothing
     Raw<T, V> rx[TS]; Raw<TG, V> rg[TS];
+    Window win{};
+    if constexpr (PACKED) { win = window_of(p, t0); __builtin_amdgcn_sched_barrier(0); }
     fetch<TG, V, TS>(p, p.gate, p.g_sb, p.g_st, q, lv * sizeof(TG), rg);
     fetch<T, V, TS>(p, p.x, p.x_sb, p.x_st, q, lt, rx);
     Marks m{0, 0, 0};
-    if constexpr (PACKED) m = marks_of<TS>(p, t0);
+    if constexpr (PACKED) m = marks_of<TS>(p, t0, win, seqs[wave]);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
     arrived(rg); arrived(rx);
     S a[TS][V], u[TS][V];                                     // (a, b) of each row
@@ -359,8 +420,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
             if ((m.start >> i) & 1) {
-                const int64_t s = seq_behind(p, t0 + i);
-                if (p.h0 && s < p.nseq) {
+                const int64_t s = uniform(seqs[wave][i]);
+                if (p.h0) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) u[i][v] += a[i][v] * ((const S*)p.h0 + (s * p.D + c0))[lv + v];
                 } else {
@@ -377,14 +438,16 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
     S A[V], H[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+    by_marks<PACKED>(m, [&](auto marked) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i)
+        for (int i = 0; i < TS; ++i)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const bool cut = PACKED && ((cuts >> i) & 1);
-            H[v] = cut ? u[i][v] : a[i][v] * H[v] + u[i][v];
-            A[v] *= a[i][v];                                  // not used where the piece is cut
-        }
+            for (int v = 0; v < V; ++v) {
+                const bool cut = marked.value && ((cuts >> i) & 1);
+                H[v] = cut ? u[i][v] : a[i][v] * H[v] + u[i][v];
+                A[v] *= a[i][v];                              // not used where the piece is cut
+            }
+    });
 #pragma unroll
     for (int v = 0; v < V; ++v) { sh.A[wave][lane * V + v] = A[v]; sh.H[wave][lane * V + v] = H[v]; }
     if (lane == 0) sh.cut[wave] = cuts != 0;
@@ -402,26 +465,28 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
         for (int v = 0; v < V; ++v) ((S*)p.ckpt + ((b * p.nckpt + t0 / TTA) * p.D + c0))[lv + v] = st[v];
     }
     T* hr = (T*)p.h + (b * p.h_sb + t0 * p.h_st + c0);
+    by_marks<PACKED>(m, [&](auto marked) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-        Pack<T, V> o;
+        for (int i = 0; i < TS; ++i) {
+            Pack<T, V> o;
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            st[v] = (PACKED && ((cuts >> i) & 1)) ? u[i][v] : a[i][v] * st[v] + u[i][v];
-            o.v[v] = (T)st[v];
-        }
-        if (on && i < rows) write<T, V>(hr, lt, o);
-        hr += p.h_st;
-        if constexpr (PACKED) {
-            if ((m.end >> i) & 1) {
-                const int64_t s = seq_behind(p, t0 + i);
-                if (on && s < p.nseq) {
+            for (int v = 0; v < V; ++v) {
+                st[v] = (marked.value && ((cuts >> i) & 1)) ? u[i][v] : a[i][v] * st[v] + u[i][v];
+                o.v[v] = (T)st[v];
+            }
+            if (on && i < rows) write<T, V>(hr, lt, o);
+            hr += p.h_st;
+            if constexpr (marked.value) {
+                if ((m.end >> i) & 1) {
+                    const int64_t s = uniform(seqs[wave][i]);
+                    if (on) {
 #pragma unroll
-                    for (int v = 0; v < V; ++v) ((S*)p.h_final + (s * p.D + c0))[lv + v] = st[v];
+                        for (int v = 0; v < V; ++v) ((S*)p.h_final + (s * p.D + c0))[lv + v] = st[v];
+                    }
                 }
             }
         }
-    }
+    });
     if constexpr (PACKED) {                                   // a sequence without rows ends where it starts
         for (int64_t s = (int64_t)k * NW + wave; s < p.nseq; s += (int64_t)p.ntiles * NW)
             if (offset_at(p, s + 1) <= offset_at(p, s) && on) {
@@ -437,11 +502,13 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 // ---- adjoint ------------------------------------------------------------------------------------------------------------------------------------------------------
 // Where 1 - a is needed, 16-bit data keep it in registers and a = 1 - (1 - a) is one instruction; wider ones keep a and evaluate the gate again at the end.  16-bit data also leave x and dh
 // as they arrived and make 32-bit values of them each time they are used (`again` hides that they are the same values), and read dh a second time, from L2: then three workgroups share
-// a CU instead of two (80 registers), and the adjoint of 8 x 4096 x 2048 BF16 takes 166 us instead of 180.
+// a CU instead of two (80 registers), and the adjoint of 8 x 4096 x 2048 BF16 takes 164 us instead of 180.  (Not for packed rows where 1 - a is kept: 13-29 registers would spill, 64-75 us
+// for 37 ... 512 sequences of 16384 x 1024 F16 against 64-80.)
 template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
-__global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && sizeof(TG) == 2 && !PACKED ? 6 : 4) k_adjoint(const Args p) {
+__global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && sizeof(TG) == 2 && !(PACKED && (COUPLED || FORM == 2)) ? 6 : 4) k_adjoint(const Args p) {
     __shared__ Lds<S, V> sh;
     constexpr int TS = TSA;
+    __shared__ int64_t seqs[PACKED ? NW : 1][TS];
     constexpr bool FAST = sizeof(T) == 2 && sizeof(TG) == 2, REST = COUPLED || FORM == 2, KEEP = REST && FAST, LATE = KEEP || !COUPLED;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const uint32_t taken = take(p, &sh.ticket);
@@ -451,6 +518,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
     const bool on = lane * V < q.channels;
     const uint32_t lv = on ? lane * V : 0, lt = lv * sizeof(T), lg = lv * sizeof(TG);
     Raw<T, V> rx[TS], rd[TS]; Raw<TG, V> rg[TS];
+    Window win{};
+    if constexpr (PACKED) { win = window_of(p, t0); __builtin_amdgcn_sched_barrier(0); }
     fetch<TG, V, TS>(p, p.gate, p.g_sb, p.g_st, q, lg, rg);
     fetch<T, V, TS>(p, p.x, p.x_sb, p.x_st, q, lt, rx);
     if (p.dh) fetch<T, V, TS>(p, p.dh, p.dh_sb, p.dh_st, q, lt, rd);
@@ -459,7 +528,7 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         for (int i = 0; i < TS; ++i) rd[i] = 0;
     }
     Marks m{0, 0, 0};
-    if constexpr (PACKED) m = marks_of<TS>(p, t0);
+    if constexpr (PACKED) m = marks_of<TS>(p, t0, win, seqs[wave]);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
     arrived(rg); arrived(rx); arrived(rd);
     S kept[TS][V], before[TS][V];                             // 1 - a (INVERSE) or a of each row; the state before it, till then its b unless that is made again from x (LATE)
@@ -478,13 +547,13 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
             for (int i = 0; i < TS; ++i) arrived(kept[i]);
     };
     auto at_seq = [&](const void* of, int i, int v) -> S {    // of the sequence that row i belongs to, in h0 or dh_final
-        const int64_t s = seq_behind(p, t0 + i);
-        return of && s < p.nseq ? ((const S*)of + (s * p.D + c0))[lv + v] : S(0);
+        const int64_t s = uniform(seqs[wave][i]);
+        return of ? ((const S*)of + (s * p.D + c0))[lv + v] : S(0);
     };
     // the cotangent of a row's state from outside the recurrence (a sequence's last row also feeds its final state); nothing in a row of no sequence
-    auto cot = [&](int i, int v) -> S {
+    auto cot = [&](auto marked, int i, int v) -> S {
         S d = (S)part<T, V>(rd[i], v);
-        if constexpr (PACKED) {
+        if constexpr (marked.value) {
             if ((m.out >> i) & 1) d = S(0);
             if ((m.end >> i) & 1) d += at_seq(p.dh_final, i, v);
         }
@@ -519,16 +588,18 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
     S A[V], H[V], F[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+    by_marks<PACKED>(m, [&](auto marked) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i)
+        for (int i = 0; i < TS; ++i)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const S ai = a(i, v);
-            S bb = (PACKED && ((m.out >> i) & 1)) ? S(0) : b_of(i, v);
-            if constexpr (PACKED) { if ((m.start >> i) & 1) bb += ai * at_seq(p.h0, i, v); }
-            H[v] = (PACKED && ((cuts >> i) & 1)) ? bb : ai * H[v] + bb;
-            A[v] *= ai;
-        }
+            for (int v = 0; v < V; ++v) {
+                const S ai = a(i, v);
+                S bb = (marked.value && ((m.out >> i) & 1)) ? S(0) : b_of(i, v);
+                if constexpr (marked.value) { if ((m.start >> i) & 1) bb += ai * at_seq(p.h0, i, v); }
+                H[v] = (marked.value && ((cuts >> i) & 1)) ? bb : ai * H[v] + bb;
+                A[v] *= ai;
+            }
+    });
 #pragma unroll
     for (int v = 0; v < V; ++v) { sh.A[wave][lane * V + v] = A[v]; sh.H[wave][lane * V + v] = H[v]; }
     if (lane == 0) sh.cut[wave] = cuts != 0;
@@ -545,11 +616,13 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
     again();
 #pragma unroll
     for (int v = 0; v < V; ++v) H[v] = S(0);
+    by_marks<PACKED>(m, [&](auto marked) {
 #pragma unroll
-    for (int i = TS - 1; i >= 0; --i) {
+        for (int i = TS - 1; i >= 0; --i) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) { const S d = cot(i, v); H[v] = (PACKED && ((cuts >> i) & 1)) ? S(0) : a(i, v) * (d + H[v]); }
-    }
+            for (int v = 0; v < V; ++v) { const S d = cot(marked, i, v); H[v] = (marked.value && ((cuts >> i) & 1)) ? S(0) : a(i, v) * (d + H[v]); }
+        }
+    });
     again();
     const int rw = NW - 1 - wave;                             // the piece's place in scan order
 #pragma unroll
@@ -573,62 +646,64 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         }
     }
     // the states before each row, then the rows from the last to the first
+    by_marks<PACKED>(m, [&](auto marked) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
+        for (int i = 0; i < TS; ++i) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            if (PACKED && ((m.start >> i) & 1)) F[v] = at_seq(p.h0, i, v);
-            const S bb = b_of(i, v);
-            before[i][v] = F[v];
-            F[v] = a(i, v) * F[v] + bb;
-            if (PACKED && ((m.out >> i) & 1)) F[v] = S(0);
-        }
-    }
-    again();
-    T* dxr = (T*)p.dx + (b * p.dx_sb + (t0 + TS - 1) * p.dx_st + c0);
-    TG* dgr = (TG*)p.dgate + (b * p.dg_sb + (t0 + TS - 1) * p.dg_st + c0);
-#pragma unroll
-    for (int i = TS - 1; i >= 0; --i) {
-        Pack<T, V> ox; Pack<TG, V> og;
-        S lastG[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            const S G = cot(i, v) + R[v], ai = a(i, v);
-            S aa, rest = S(1);
-            if constexpr (KEEP) rest = rest_of(i, v);
-            else if constexpr (REST) decay<FORM, true, FAST, S>((S)part<TG, V>(rg[i], v), aa, rest);
-            S da = G * (COUPLED ? before[i][v] - (S)part<T, V>(rx[i], v) : before[i][v]);
-            if constexpr (FORM == 1) da *= ai;
-            if constexpr (FORM == 2) da *= ai * rest;
-            S dx = COUPLED ? G * rest : G;
-            R[v] = ai * G;
-            lastG[v] = G;
-            if (PACKED && ((m.out >> i) & 1)) { da = S(0); dx = S(0); R[v] = S(0); }
-            ox.v[v] = (T)dx; og.v[v] = (TG)da;
-        }
-        if (on && i < rows) {
-            if (p.dx) write<T, V>(dxr, lt, ox);
-            if (p.dgate) write<TG, V>(dgr, lg, og);
-        }
-        dxr -= p.dx_st; dgr -= p.dg_st;
-        // the gradient of a start leaves in the state's type: 1 - (1 - a) would not do for a small a
-        if (INVERSE && (PACKED ? (m.start >> i) & 1 : i == 0 && tile == 0 && wave == 0)) {
-            const Raw<TG, V> g0 = read<TG, V>((const TG*)p.gate + (b * p.g_sb + (t0 + i) * p.g_st + c0), lg);
-#pragma unroll
-            for (int v = 0; v < V; ++v) { S aa, rest; decay<FORM, false, FAST, S>((S)part<TG, V>(g0, v), aa, rest); R[v] = aa * lastG[v]; }
-        }
-        if constexpr (PACKED) {
-            if ((m.start >> i) & 1) {
-                const int64_t s = seq_behind(p, t0 + i);
-                if (on && p.dh0 && s < p.nseq) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) ((S*)p.dh0 + (s * p.D + c0))[lv + v] = R[v];
-                }
-#pragma unroll
-                for (int v = 0; v < V; ++v) R[v] = S(0);
+            for (int v = 0; v < V; ++v) {
+                if (marked.value && ((m.start >> i) & 1)) F[v] = at_seq(p.h0, i, v);
+                const S bb = b_of(i, v);
+                before[i][v] = F[v];
+                F[v] = a(i, v) * F[v] + bb;
+                if (marked.value && ((m.out >> i) & 1)) F[v] = S(0);
             }
         }
-    }
+        again();
+        T* dxr = (T*)p.dx + (b * p.dx_sb + (t0 + TS - 1) * p.dx_st + c0);
+        TG* dgr = (TG*)p.dgate + (b * p.dg_sb + (t0 + TS - 1) * p.dg_st + c0);
+#pragma unroll
+        for (int i = TS - 1; i >= 0; --i) {
+            Pack<T, V> ox; Pack<TG, V> og;
+            S lastG[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const S G = cot(marked, i, v) + R[v], ai = a(i, v);
+                S aa, rest = S(1);
+                if constexpr (KEEP) rest = rest_of(i, v);
+                else if constexpr (REST) decay<FORM, true, FAST, S>((S)part<TG, V>(rg[i], v), aa, rest);
+                S da = G * (COUPLED ? before[i][v] - (S)part<T, V>(rx[i], v) : before[i][v]);
+                if constexpr (FORM == 1) da *= ai;
+                if constexpr (FORM == 2) da *= ai * rest;
+                S dx = COUPLED ? G * rest : G;
+                R[v] = ai * G;
+                lastG[v] = G;
+                if (marked.value && ((m.out >> i) & 1)) { da = S(0); dx = S(0); R[v] = S(0); }
+                ox.v[v] = (T)dx; og.v[v] = (TG)da;
+            }
+            if (on && i < rows) {
+                if (p.dx) write<T, V>(dxr, lt, ox);
+                if (p.dgate) write<TG, V>(dgr, lg, og);
+            }
+            dxr -= p.dx_st; dgr -= p.dg_st;
+            // the gradient of a start leaves in the state's type: 1 - (1 - a) would not do for a small a
+            if (INVERSE && (marked.value ? (m.start >> i) & 1 : !PACKED && i == 0 && tile == 0 && wave == 0)) {
+                const Raw<TG, V> g0 = read<TG, V>((const TG*)p.gate + (b * p.g_sb + (t0 + i) * p.g_st + c0), lg);
+#pragma unroll
+                for (int v = 0; v < V; ++v) { S aa, rest; decay<FORM, false, FAST, S>((S)part<TG, V>(g0, v), aa, rest); R[v] = aa * lastG[v]; }
+            }
+            if constexpr (marked.value) {
+                if ((m.start >> i) & 1) {
+                    const int64_t s = uniform(seqs[wave][i]);
+                    if (on && p.dh0) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) ((S*)p.dh0 + (s * p.D + c0))[lv + v] = R[v];
+                    }
+#pragma unroll
+                    for (int v = 0; v < V; ++v) R[v] = S(0);
+                }
+            }
+        }
+    });
     if constexpr (PACKED) {
         for (int64_t s = (int64_t)k * NW + wave; s < p.nseq; s += (int64_t)p.ntiles * NW)
             if (offset_at(p, s + 1) <= offset_at(p, s) && on && p.dh0) {

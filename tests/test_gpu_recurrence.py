@@ -97,6 +97,18 @@ def test_long_axis_of_many_groups(sa, torch):
     compare(sa, torch, inputs(torch, 6, (1, 9000, 5), 1, "log", "float32"), "log", False, "float32")
 
 
+# one or two, three or four and more chains (of 64 float32 channels): groups of 32, 16 and 8 tiles of 128 rows (adjoint: 64), whole ones and one row more; float64 publishes in other words
+@pytest.mark.parametrize("channels", [70, 200, 330])
+@pytest.mark.parametrize("length", [2048, 2049, 4096, 4225])
+def test_groups_of_tiles_by_the_number_of_chains(sa, torch, channels, length):
+    compare(sa, torch, inputs(torch, 26, (1, length, channels), 1, "log", "float32"), "log", True, "float32")
+
+
+@pytest.mark.parametrize("channels", [64, 192, 320])
+def test_groups_of_tiles_in_64_bits(sa, torch, channels):
+    compare(sa, torch, inputs(torch, 27, (1, 4100, channels), 1, "sigmoid", "float64"), "sigmoid", True, "float64")
+
+
 PACKS = [[0, 5], [0, 0, 1, 1, 40], [0, 16, 32, 128, 128, 128, 300], [3, 70, 70, 71, 200, 290], [0, 1, 2, 3, 4, 5, 6, 7, 8, 20, 300], [0, 0, 0], [300, 300], [0, 300], [64, 128, 192, 256]]
 
 
@@ -114,6 +126,17 @@ def test_packed_many_sequences_and_64_bit_offsets(sa, torch):
     sol, grads = compare(sa, torch, q, "log", True, "float32", offsets=offsets)
     again = sa.recurrence_solve(q["x"], q["gate"], q["h0"], form="log", coupled=True, offsets=torch.tensor(offsets, dtype=torch.int64, device="cuda"))
     assert torch.equal(again.h, sol.h) and torch.equal(again.h_final, sol.h_final)
+
+
+# a wave looks at 64 sequences together: more empty ones than that between two rows of a piece, before the first and behind the last; 64, 65 and 4096 and more sequences of a row or none
+EMPTY = [[0, 3] + [9] * 70 + [12, 300], [0] * 130 + [5, 300], [0, 200] + [300] * 200, [0] + [40] * 63 + [41], [0] + [40] * 64 + [41], list(range(0, 65)), list(range(0, 301)),
+         [0] + [i // 16 for i in range(4800)] + [300]]
+
+
+@pytest.mark.parametrize("offsets", EMPTY, ids=[str(i) for i in range(len(EMPTY))])
+@pytest.mark.parametrize("dtype,coupled,form", [("bfloat16", False, "log"), ("float32", True, "sigmoid")])
+def test_packed_windows_of_empty_sequences(sa, torch, offsets, dtype, coupled, form):
+    compare(sa, torch, inputs(torch, 28, (300, 6), len(offsets) - 1, form, dtype), form, coupled, dtype, offsets=offsets)
 
 
 def test_nothing_leaks_between_sequences(sa, torch):
