@@ -157,12 +157,13 @@ template <class T, bool SPLIT, int WAVES> __global__ void __launch_bounds__(WAVE
 // Bound: the matrix cores, at the clock that the board's power leaves (1.95 GHz while they are busy).  4096 x 4096, one term: X X' and the polynomial of A, half their tiles each, 92 and 96 us
 // (750 and 715 TFLOP/s of the half), B X with X out in three forms 147-163 us (840-930).  Small sides: a launch of 4-9 us each, most of it the latency of the first stages and of the
 // epilogue (two groups of four waves that share a tile and halve K were 10 % slower at every size).
-enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3 };
+enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3, PARTS = 4, JOIN = 5 };        // PARTS, JOIN: GRAM in two launches, parts of K and their sum (in the order of the parts)
 
 struct Product {
     const f16 *P[2], *Q[2];                   // terms
     int64_t sP, sQ;                           // matrix strides
     int64_t K, M, N;                          // padded: P [M][K], Q [N][K]
+    int tiles, parts;                         // PARTS, JOIN: tiles of a matrix, parts of K
     float c0, c1, c2;
     bool rounded;                             // APPLY, LAST: X in c0 X is the rounded one
     bool keep;                                // APPLY: the next step needs the F32 X
@@ -193,15 +194,18 @@ __global__ void __launch_bounds__(256, BT == 64 || (BT == 128 && SLOTS == 1) ? 2
     __shared__ __align__(16) f16 s0[BUF], s1[BUF], s2[BUF], s3[BUF];
     const int64_t b = blockIdx.z;
     int bi, bj;
-    if constexpr (EPI == GRAM || EPI == POLY) {               // tile t of the lower triangle
-        const int t = blockIdx.x;
+    constexpr bool LOWER = EPI != APPLY && EPI != LAST;
+    int tile = (int)blockIdx.x, part = 0;
+    if constexpr (EPI == PARTS) { tile = (int)(blockIdx.x % (uint32_t)g.tiles); part = (int)(blockIdx.x / (uint32_t)g.tiles); }
+    if constexpr (LOWER) {                                    // tile t of the lower triangle
+        const int t = tile;
         bi = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
         while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
         while (bi * (bi + 1) / 2 > t) --bi;
         bj = t - bi * (bi + 1) / 2;
     } else {
         // workgroups go round the eight XCDs: each gets a compact part of the tiles (2 x 4 parts), so that its L2 serves its factors' rows to all of them
-        const int ti = (int)((g.M + BT - 1) / BT), tj = (int)((g.N + BT - 1) / BT), t = blockIdx.x;
+        const int ti = (int)((g.M + BT - 1) / BT), tj = (int)((g.N + BT - 1) / BT), t = tile;
         if (ti % 2 == 0 && tj % 4 == 0) {
             const int x = t & 7, u = t >> 3, wj4 = tj / 4;
             bi = (x >> 2) * (ti / 2) + u / wj4; bj = (x & 3) * wj4 + u % wj4;
@@ -216,89 +220,117 @@ __global__ void __launch_bounds__(256, BT == 64 || (BT == 128 && SLOTS == 1) ? 2
         for (int y = 0; y < W; ++y)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[x][y][r] = 0.f;
-    constexpr int DEPTH = SPLIT ? BK : SLOTS * BK;            // of a stage, in k
-    const int stages = (int)(g.K / DEPTH);                    // a multiple of four, or of two
-    // rows past the last one (the sides are multiples of 128, not of every BT) are requested from the last one, multiplied and not stored
-    int64_t row_p[RQ], row_q[RQ];
+    // sums of part p of a tile, F32: an accumulator's registers four at a time, lanes next to each other
+    f32x4* const parts = (f32x4*)(q.xt[to][0] + b * q.np * q.mp) + (int64_t)tile * (W * W * 1024) + wave * 256 + lane;
+    const int64_t part_step = (int64_t)g.tiles * (W * W * 1024);
+    if constexpr (EPI == JOIN) {
+        for (int p = 0; p < g.parts; ++p)
 #pragma unroll
-    for (int c = 0; c < RQ; ++c) {
-        const int64_t r = (wave * RQ + c) * 16 + (lane >> 2), k = ((lane & 3) ^ ((lane >> 4) & 3)) * 8;
-        row_p[c] = (i0 + r < g.M ? i0 + r : g.M - 1) * g.K + k;
-        row_q[c] = (j0 + r < g.N ? j0 + r : g.N - 1) * g.K + k;
-    }
-    // request n of the 2 SLOTS RQ of a stage; behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
-    constexpr int NREQ = 2 * SLOTS * RQ;
-    auto request = [&](int s, f16* buf, int n) {
-        s = s < stages ? s : stages - 1;
-        const int slice = n / RQ, c = n % RQ, slot = slice % SLOTS, term = SPLIT ? slot : 0;
-        const int k = s * DEPTH + (SPLIT ? 0 : slot * BK);
-        const f16* from = slice < SLOTS ? g.P[term] + b * g.sP + k + row_p[c] : g.Q[term] + b * g.sQ + k + row_q[c];
-        __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                         (__attribute__((address_space(3))) void*)(buf + slice * SLICE + (wave * RQ + c) * 512), 16, 0, 0);
-    };
-    const int rp = (wi * (BT / 2) + (lane & 31)) * BK, rq = SLOTS * SLICE + (wj * (BT / 2) + (lane & 31)) * BK;
-    const int ch0 = ((lane >> 5) ^ ((lane >> 2) & 3)) * 8, ch1 = ((2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 8;
-    typedef f16x8 Factors[SLOTS][2][W];                       // [slot][P, Q]
-    constexpr int NREAD = 2 * SLOTS * W;
-    Factors f0, f1;
-    auto read = [&](const f16* buf, int ch, Factors& f, int n) {
-        const int slot = n / (2 * W), which = n / W % 2, x = n % W;
-        f[slot][which][x] = *(const f16x8*)(buf + slot * SLICE + (which ? rq : rp) + x * 32 * BK + ch);
-    };
-    // half a stage: the products of one half with the reads of the next and half a stage's requests between them, one at a time — issued in a burst they hold the wave, and with it the
-    // matrix core, up to the rate of the request queue and of LDS
-    constexpr int SETS = SPLIT ? 3 : SLOTS, NM = SETS * W * W;
-    auto half = [&](const Factors& f, const f16* rbuf, int ch, Factors& nf, int rs, f16* qbuf, int n0) {
-        int reads = 0, requests = 0;
+            for (int x = 0; x < W; ++x)
 #pragma unroll
-        for (int m = 0; m < NM; ++m) {
-            const int set = m / (W * W), x = m / W % W, y = m % W;
-            const int tp = SPLIT ? set == 1 : set, tq = SPLIT ? set == 0 : set;    // split: hi lo, lo hi, hi hi
-            acc[x][y] = mfma(f[tp][0][x], f[tq][1][y], acc[x][y]);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int y = 0; y < W; ++y)
 #pragma unroll
-            for (; reads < NREAD && reads * 2 * NM < (m + 1) * NREAD * 3; ++reads) read(rbuf, ch, nf, reads);     // all within the first two thirds
+                    for (int h = 0; h < 4; ++h) {
+                        const f32x4 v = parts[p * part_step + (x * W + y) * 1024 + h * 64];
 #pragma unroll
-            for (; requests < NREQ / 2 && (requests + 1) * NM <= (m + 1) * (NREQ / 2); ++requests) request(rs, qbuf, n0 + requests);
-            __builtin_amdgcn_sched_barrier(0);
+                        for (int r = 0; r < 4; ++r) acc[x][y][h * 4 + r] += v[r];
+                    }
+    } else {
+        const int64_t nk = g.K / PADDED, k0 = EPI == PARTS ? nk * part / g.parts * PADDED : 0, k1 = EPI == PARTS ? nk * (part + 1) / g.parts * PADDED : g.K;
+        constexpr int DEPTH = SPLIT ? BK : SLOTS * BK;            // of a stage, in k
+        const int stages = (int)((k1 - k0) / DEPTH);              // a multiple of four, or of two
+        // rows past the last one (the sides are multiples of 128, not of every BT) are requested from the last one, multiplied and not stored
+        int64_t row_p[RQ], row_q[RQ];
+#pragma unroll
+        for (int c = 0; c < RQ; ++c) {
+            const int64_t r = (wave * RQ + c) * 16 + (lane >> 2), k = k0 + ((lane & 3) ^ ((lane >> 4) & 3)) * 8;
+            row_p[c] = (i0 + r < g.M ? i0 + r : g.M - 1) * g.K + k;
+            row_q[c] = (j0 + r < g.N ? j0 + r : g.N - 1) * g.K + k;
         }
-    };
-    // the oldest stage in flight has arrived in this wave's part (those of two later ones may still be on the way) and its LDS reads are done; then in all waves
-    auto arrive = [&]() {
-        static_assert(NREQ == 4 || NREQ == 6 || NREQ == 8, "the counts below");
-        __builtin_amdgcn_s_waitcnt(NREQ == 8 ? 0x4070 : NREQ == 6 ? 0x007c : 0x0078);        // vmcnt(2 NREQ) lgkmcnt(0)
-        __builtin_amdgcn_s_barrier();
+        // request n of the 2 SLOTS RQ of a stage; behind the last stage the last one once more, into a buffer that is not read again: the counts stay the same
+        constexpr int NREQ = 2 * SLOTS * RQ;
+        auto request = [&](int s, f16* buf, int n) {
+            s = s < stages ? s : stages - 1;
+            const int slice = n / RQ, c = n % RQ, slot = slice % SLOTS, term = SPLIT ? slot : 0;
+            const int k = s * DEPTH + (SPLIT ? 0 : slot * BK);
+            const f16* from = slice < SLOTS ? g.P[term] + b * g.sP + k + row_p[c] : g.Q[term] + b * g.sQ + k + row_q[c];
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                             (__attribute__((address_space(3))) void*)(buf + slice * SLICE + (wave * RQ + c) * 512), 16, 0, 0);
+        };
+        const int rp = (wi * (BT / 2) + (lane & 31)) * BK, rq = SLOTS * SLICE + (wj * (BT / 2) + (lane & 31)) * BK;
+        const int ch0 = ((lane >> 5) ^ ((lane >> 2) & 3)) * 8, ch1 = ((2 + (lane >> 5)) ^ ((lane >> 2) & 3)) * 8;
+        typedef f16x8 Factors[SLOTS][2][W];                       // [slot][P, Q]
+        constexpr int NREAD = 2 * SLOTS * W;
+        Factors f0, f1;
+        auto read = [&](const f16* buf, int ch, Factors& f, int n) {
+            const int slot = n / (2 * W), which = n / W % 2, x = n % W;
+            f[slot][which][x] = *(const f16x8*)(buf + slot * SLICE + (which ? rq : rp) + x * 32 * BK + ch);
+        };
+        // half a stage: the products of one half with the reads of the next and half a stage's requests between them, one at a time — issued in a burst they hold the wave, and with it the
+        // matrix core, up to the rate of the request queue and of LDS
+        constexpr int SETS = SPLIT ? 3 : SLOTS, NM = SETS * W * W;
+        auto half = [&](const Factors& f, const f16* rbuf, int ch, Factors& nf, int rs, f16* qbuf, int n0) {
+            int reads = 0, requests = 0;
+#pragma unroll
+            for (int m = 0; m < NM; ++m) {
+                const int set = m / (W * W), x = m / W % W, y = m % W;
+                const int tp = SPLIT ? set == 1 : set, tq = SPLIT ? set == 0 : set;    // split: hi lo, lo hi, hi hi
+                acc[x][y] = mfma(f[tp][0][x], f[tq][1][y], acc[x][y]);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (; reads < NREAD && reads * 2 * NM < (m + 1) * NREAD * 3; ++reads) read(rbuf, ch, nf, reads);     // all within the first two thirds
+#pragma unroll
+                for (; requests < NREQ / 2 && (requests + 1) * NM <= (m + 1) * (NREQ / 2); ++requests) request(rs, qbuf, n0 + requests);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // the oldest stage in flight has arrived in this wave's part (those of two later ones may still be on the way) and its LDS reads are done; then in all waves
+        auto arrive = [&]() {
+            static_assert(NREQ == 4 || NREQ == 6 || NREQ == 8, "the counts below");
+            __builtin_amdgcn_s_waitcnt(NREQ == 8 ? 0x4070 : NREQ == 6 ? 0x007c : 0x0078);        // vmcnt(2 NREQ) lgkmcnt(0)
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        // behind the barrier no wave reads `now` any more: its next stage is requested half there, half in the first half of the next stage
+        auto stage = [&](int s, f16* prev, f16* now, const f16* next) {
+            half(f0, now, ch1, f1, s + 3, prev, NREQ / 2);
+            arrive();
+            half(f1, next, ch0, f0, s + 4, now, 0);
+        };
+        auto all = [&](int s, f16* buf, int from, int to) {
+#pragma unroll
+            for (int n = from; n < to; ++n) request(s, buf, n);
+        };
+        all(0, s0, 0, NREQ); all(1, s1, 0, NREQ); all(2, s2, 0, NREQ);
         __builtin_amdgcn_sched_barrier(0);
-    };
-    // behind the barrier no wave reads `now` any more: its next stage is requested half there, half in the first half of the next stage
-    auto stage = [&](int s, f16* prev, f16* now, const f16* next) {
-        half(f0, now, ch1, f1, s + 3, prev, NREQ / 2);
         arrive();
-        half(f1, next, ch0, f0, s + 4, now, 0);
-    };
-    auto all = [&](int s, f16* buf, int from, int to) {
+        all(3, s3, 0, NREQ / 2);
 #pragma unroll
-        for (int n = from; n < to; ++n) request(s, buf, n);
-    };
-    all(0, s0, 0, NREQ); all(1, s1, 0, NREQ); all(2, s2, 0, NREQ);
-    __builtin_amdgcn_sched_barrier(0);
-    arrive();
-    all(3, s3, 0, NREQ / 2);
-#pragma unroll
-    for (int n = 0; n < NREAD; ++n) read(s0, ch0, f0, n);
-    int s = 0;
-    for (; s + 4 <= stages; s += 4) {
-        stage(s, s3, s0, s1);
-        stage(s + 1, s0, s1, s2);
-        stage(s + 2, s1, s2, s3);
-        stage(s + 3, s2, s3, s0);
-    }
-    if constexpr (SLOTS == 2 && !SPLIT)                       // K is a multiple of 128: two stages of 64 may be left
-        if (s < stages) {
+        for (int n = 0; n < NREAD; ++n) read(s0, ch0, f0, n);
+        int s = 0;
+        for (; s + 4 <= stages; s += 4) {
             stage(s, s3, s0, s1);
             stage(s + 1, s0, s1, s2);
+            stage(s + 2, s1, s2, s3);
+            stage(s + 3, s2, s3, s0);
         }
-    __builtin_amdgcn_s_waitcnt(0x0070);                       // nothing is on the way to LDS when the workgroup ends
+        if constexpr (SLOTS == 2 && !SPLIT)                       // K is a multiple of 128: two stages of 64 may be left
+            if (s < stages) {
+                stage(s, s3, s0, s1);
+                stage(s + 1, s0, s1, s2);
+            }
+        __builtin_amdgcn_s_waitcnt(0x0070);                       // nothing is on the way to LDS when the workgroup ends
+    }
+    if constexpr (EPI == PARTS) {
+#pragma unroll
+        for (int x = 0; x < W; ++x)
+#pragma unroll
+            for (int y = 0; y < W; ++y)
+#pragma unroll
+                for (int h = 0; h < 4; ++h)
+                    parts[part * part_step + (x * W + y) * 1024 + h * 64] = f32x4{acc[x][y][h * 4], acc[x][y][h * 4 + 1], acc[x][y][h * 4 + 2], acc[x][y][h * 4 + 3]};
+        return;
+    }
     // A lane holds, of each 32 x 32, column lane & 31 and rows 8 g + 4 (lane >> 5) + 0..3 for g = 0..3: four neighbours of the transposed order.  For the other order four lanes
     // exchange theirs, so that both are stored eight bytes at a time.  What a row of accumulators needs from memory is requested before any of it is used.
     const int64_t jw = j0 + wj * (BT / 2) + (lane & 31), iw = i0 + wi * (BT / 2) + (lane >> 5) * 4;
@@ -357,7 +389,7 @@ __global__ void __launch_bounds__(256, BT == 64 || (BT == 128 && SLOTS == 1) ? 2
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     v[r] = acc[x][y][h * 4 + r];
-                    if constexpr (EPI == GRAM) v[r] *= SA / (SX * SX);
+                    if constexpr (EPI == GRAM || EPI == JOIN) v[r] *= SA / (SX * SX);
                     else if constexpr (EPI == POLY) v[r] = g.c1 * old[y][h][r] + g.c2 * (v[r] * (1.f / SA));
                     else v[r] = g.c0 * old[y][h][r] + v[r] * (1.f / SA);
                 }
@@ -397,9 +429,9 @@ __global__ void __launch_bounds__(256, BT == 64 || (BT == 128 && SLOTS == 1) ? 2
                     f16x4 hi, lo;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) { f16 e, l = 0; terms<SPLIT>(v[r], e, l); hi[r] = e; lo[r] = l; }
-                    constexpr bool SQUARE = EPI == GRAM || EPI == POLY;
-                    f16* const* direct = EPI == GRAM ? q.a : EPI == POLY ? q.b : q.x;
-                    f16* const* turned = EPI == GRAM ? q.a : EPI == POLY ? q.b : q.xt[to];
+                    constexpr bool SQUARE = LOWER;
+                    f16* const* direct = EPI == POLY ? q.b : SQUARE ? q.a : q.x;
+                    f16* const* turned = EPI == POLY ? q.b : SQUARE ? q.a : q.xt[to];
                     const int64_t att = SQUARE ? (b * q.mp + j) * q.mp + i : (b * q.np + j) * q.mp + i;
                     const int64_t atd = SQUARE ? (b * q.mp + i + quad) * q.mp + j - quad : (b * q.mp + i + quad) * q.np + j - quad;
                     *(f16x4*)(turned[0] + att) = hi;

@@ -48,7 +48,7 @@ static int64_t tiles_of(const Product& g, int64_t batch, bool lower, int64_t BT)
     return (lower ? ti * (ti + 1) / 2 : ti * tj) * batch;
 }
 template <class T, int BT, int EPI, bool SPLIT, int SLOTS> static void product(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
-    const dim3 grid((uint32_t)tiles_of(g, 1, EPI == GRAM || EPI == POLY, BT), 1, (uint32_t)q.batch);
+    const dim3 grid((uint32_t)(tiles_of(g, 1, EPI != APPLY && EPI != LAST, BT) * (EPI == PARTS ? g.parts : 1)), 1, (uint32_t)q.batch);
     k_product<T, BT, EPI, SPLIT, SLOTS><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
 }
 
@@ -59,22 +59,35 @@ template <class T, int BT, int EPI, bool SPLIT, int SLOTS> static void product(c
 struct TileCost { int BT; double fixed, round, row, load; };
 static constexpr TileCost ONE_TERM[] = {{64, 2.0, 2.2, 3.0e-3, 0.5}, {128, 2.0, 3.5, 6.0e-3, 0.65}, {192, 3.0, 8.0, 9.8e-3, 0.9}, {256, 4.0, 14.0, 16.3e-3, 0.9}};
 static constexpr TileCost TWO_TERMS[] = {{64, 2.0, 2.5, 7.5e-3, 0.2}, {128, 3.0, 7.5, 13.0e-3, 0.5}};
-template <int N> static int best_tile(const TileCost (&table)[N], const Product& g, int64_t batch, bool lower) {
-    int best = 0;
-    double least = 0;
-    for (const TileCost& c : table) {
-        const int64_t n = tiles_of(g, batch, lower, c.BT), rounds = (n + 255) / 256;
-        const double t = c.fixed + (double)rounds * (c.round + (double)g.K * c.row * (1.0 + c.load * (double)n / (256.0 * (double)rounds)));
-        if (!best || t < least) { best = c.BT; least = t; }
+static double cost_of(const TileCost& c, const Product& g, int64_t batch, bool lower, int parts) {
+    const int64_t n = tiles_of(g, batch, lower, c.BT) * parts, rounds = (n + 255) / 256;
+    return c.fixed + (double)rounds * (c.round + (double)g.K / parts * c.row * (1.0 + c.load * (double)n / (256.0 * (double)rounds)));
+}
+template <int N> static const TileCost& best_tile(const TileCost (&table)[N], const Product& g, int64_t batch, bool lower) {
+    const TileCost* best = table;
+    for (const TileCost& c : table) if (cost_of(c, g, batch, lower, 1) < cost_of(*best, g, batch, lower, 1)) best = &c;
+    return *best;
+}
+// X X' of few rows and long ones has few tiles: its K is cut into parts, whose sums lie where the next X will (not in use then, and large enough where the parts are worth it) and are
+// joined by a launch of its own, about 2 + 0.4 a part us.  Measured, with the join: 256 x 16384 bf16 48 us without, 30 / 19 / 15 with 2 / 4 / 8 parts; 512 x 8192 26, 20 / 16 / 19;
+// 512 x 8192 F32 58, 37 / 26 / 32; 256 x 1024 6.2, 8.6 with two.  (Tiles of 128 in parts were no faster for 2048 x 8192: 68, 80 / 71 with 2 / 3.)
+template <bool SPLIT> static int parts_of(const Product& g, const Mat& q) {
+    const TileCost& small = SPLIT ? TWO_TERMS[0] : ONE_TERM[0];
+    double least = 0.9 * (SPLIT ? cost_of(best_tile(TWO_TERMS, g, q.batch, true), g, q.batch, true, 1) : cost_of(best_tile(ONE_TERM, g, q.batch, true), g, q.batch, true, 1));
+    int best = 1;
+    for (int parts = 2; parts <= 8; parts *= 2) {
+        if (parts > g.K / PADDED || parts * tiles_of(g, 1, true, 64) * 64 * 64 * 2 > q.mp * q.np) break;
+        const double t = cost_of(small, g, q.batch, true, parts) + 2.0 + 0.4 * parts;
+        if (t < least) { least = t; best = parts; }
     }
     return best;
 }
 template <class T, int EPI, bool SPLIT> static void product_of(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
     constexpr bool LOWER = EPI == GRAM || EPI == POLY;
     if constexpr (SPLIT) {
-        if (best_tile(TWO_TERMS, g, q.batch, LOWER) == 64) product<T, 64, EPI, true, 2>(g, q, io, from, to, s);
+        if (best_tile(TWO_TERMS, g, q.batch, LOWER).BT == 64) product<T, 64, EPI, true, 2>(g, q, io, from, to, s);
         else product<T, 128, EPI, true, 2>(g, q, io, from, to, s);
-    } else switch (best_tile(ONE_TERM, g, q.batch, LOWER)) {
+    } else switch (best_tile(ONE_TERM, g, q.batch, LOWER).BT) {
         case 64: product<T, 64, EPI, false, 2>(g, q, io, from, to, s); break;
         case 128: product<T, 128, EPI, false, 1>(g, q, io, from, to, s); break;
         case 192: product<T, 192, EPI, false, 1>(g, q, io, from, to, s); break;
@@ -99,7 +112,12 @@ template <class T, bool SPLIT> static void iterate(const hipadj_orthogonal* o, c
         Product g{};
         g.c0 = (float)c[0]; g.c1 = (float)c[1]; g.c2 = (float)c[2];
         g.P[0] = g.Q[0] = q.x[0]; g.P[1] = g.Q[1] = q.x[1]; g.sP = g.sQ = smn; g.K = q.np; g.M = g.N = q.mp;
-        product_of<T, GRAM, SPLIT>(g, q, io, from, to, s);
+        g.parts = parts_of<SPLIT>(g, q);
+        if (g.parts > 1) {
+            g.tiles = (int)tiles_of(g, 1, true, 64);
+            product<T, 64, PARTS, SPLIT, 2>(g, q, io, from, to, s);
+            product<T, 64, JOIN, SPLIT, 2>(g, q, io, from, to, s);
+        } else product_of<T, GRAM, SPLIT>(g, q, io, from, to, s);
         g.P[0] = g.Q[0] = q.a[0]; g.P[1] = g.Q[1] = q.a[1]; g.sP = g.sQ = smm; g.K = q.mp;
         product_of<T, POLY, SPLIT>(g, q, io, from, to, s);
         g.P[0] = q.b[0]; g.P[1] = q.b[1]; g.sP = smm;

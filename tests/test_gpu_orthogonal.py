@@ -52,6 +52,17 @@ def test_shapes_and_types(sa, torch, shape, dtype):
     near(got, host(g), dtype, one_term=dtype == "bfloat16" and min(shape) >= 256)
 
 
+# few rows and long ones: X X' is summed in parts
+@pytest.mark.parametrize("shape,dtype", [((200, 2900), "float32"), ((2900, 200), "bfloat16"), ((256, 4200), "bfloat16"), ((2, 300, 5000), "float16"), ((9000, 130), "float32"),
+                                         ((3, 16400, 256), "bfloat16")])
+def test_long_rows(sa, torch, shape, dtype):
+    g = gradient(torch, 3, shape, dtype)
+    got, again = sa.orthogonalized_update(g), sa.orthogonalized_update(g)
+    assert torch.equal(got, again)
+    for a, b in zip(got.reshape(-1, *shape[-2:]), g.reshape(-1, *shape[-2:])):
+        near(a, host(b), dtype, one_term=dtype == "bfloat16" and min(shape[-2:]) >= 256)
+
+
 @pytest.mark.parametrize("shape", [(256, 256), (700, 300), (384, 1500), (1024, 1024)])
 def test_one_term_products(sa, torch, shape):
     g = gradient(torch, 2, shape, "bfloat16")
