@@ -150,7 +150,9 @@ _function = None
 
 
 def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=None):
-    """(h, h_final) of the gated linear recurrence (recurrence_solve), differentiable by torch's autograd with respect to x, gate and h0; first derivatives."""
+    """(h, h_final) of the gated linear recurrence (recurrence_solve), differentiable by torch's autograd with respect to x, gate and h0; first derivatives.
+    Forward and backward can be captured into a graph; as with any function of torch's autograd, no eager result of the same leaves may be alive at the capture (the engine would
+    wait for the eager pass's stream inside it)."""
     global _function
     torch = _torch()
     if _function is None:
@@ -180,7 +182,7 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
 def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=None):
     """One step of running sequences: state[slots[i]] <- a state[slots[i]] + b in place, and h[i] = the new state in x's type.  x, gate [batch][channels]; state
     [nslots][channels] float32 (float64 for float64); slots int32 / int64 [batch] or None (row i has state i).  A slot outside the states (-1) pads the batch: h[i] = 0.
-    Rows with the same slot are consecutive steps of that state in row order."""
+    Rows with the same slot are consecutive steps of that state in row order.  No gradients: gated_recurrence over one row has them."""
     torch = _torch()
     if x.dim() != 2:
         raise ValueError(f"x must be [batch][channels], got shape {tuple(x.shape)}")

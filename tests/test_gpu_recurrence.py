@@ -352,6 +352,39 @@ def test_captured_replays_and_other_streams(sa, torch):
     assert all(torch.equal(a, b) for r in results for a, b in zip(r, want))
 
 
+def test_training_step_captured_into_a_graph(sa, torch):
+    """Forward and backward of torch's autograd in one graph, dense and packed: every replay, with eager work between, leaves the gradients of the adjoint itself."""
+    q = inputs(torch, 29, (300, 70), 3, "log", "bfloat16")
+    off = torch.tensor([2, 100, 230, 290], dtype=torch.int32, device="cuda")
+    leaves = [q[k].clone().requires_grad_() for k in ("x", "gate", "h0")]
+    def dense(x, g, h0): return sa.gated_recurrence(x[None], g[None], h0[:1], coupled=True)
+    def packed(x, g, h0): return sa.gated_recurrence(x, g, h0, coupled=True, offsets=off)
+    def step():
+        out = []
+        for f in (dense, packed):
+            h, last = f(*leaves)
+            out += torch.autograd.grad([h, last], leaves, [q["dh"].reshape(h.shape), q["dhf"][:last.shape[0]]])
+        return out
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(4):
+        with torch.no_grad():
+            leaves[0].copy_(torch.randn(q["x"].shape, device="cuda", generator=torch.Generator("cuda").manual_seed(i)))
+        graph.replay()
+        x, g, h0 = (t.detach() for t in leaves)
+        a = sa.recurrence_adjoint(sa.recurrence_solve(x[None], g[None], h0[:1], coupled=True), q["dh"][None], q["dhf"][:1])
+        b = sa.recurrence_adjoint(sa.recurrence_solve(x, g, h0, coupled=True, offsets=off), q["dh"], q["dhf"])
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], a[0][0]) and torch.equal(got[1], a[1][0]) and torch.equal(got[2][:1], a[2]) and not got[2][1:].any(), i
+        assert all(torch.equal(u, v) for u, v in zip(got[3:], b)), i
+
+
 def test_offsets_past_32_bits(sa, torch):
     """Rows 2^31 elements apart: the addresses of the second batch row do not fit 32 bits."""
     far = torch.empty(2 ** 31 + 4096, dtype=torch.bfloat16, device="cuda")
