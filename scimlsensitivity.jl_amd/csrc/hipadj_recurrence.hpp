@@ -118,23 +118,23 @@ __device__ inline uint32_t await_value(const uint64_t* w, int64_t cw, double& v)
     v = __longlong_as_double((long long)((q & 0xffffffffu) | (r << 32)));
     return (uint32_t)(q >> 32);
 }
-// A map (A, H); CUT: no state passes (a sequence starts inside), H alone counts, whatever A and the state are.  In 32 bits it is one word: the last bit of A is set for "present", which
-// moves A by at most 2^-23 of itself.  1 (the smallest denormal) is CUT, 3 stands for zero — a state times it is nothing, but a NaN stays one — and the largest number for infinity.
+// A map (A, H); CUT: no state passes (a sequence starts inside), H alone counts, whatever A and the state are.  In 32 bits it is one word, and every A but the payload of a NaN passes
+// exactly (a held state is multiplied by the A of each tile: one that is off by a last bit would let it grow along the axis): the bits of A are inverted, so that the two patterns
+// that no NaN is stored as stand for "absent" (a zeroed word) and for CUT.
 constexpr uint32_t TAG_VALUE = 1, TAG_CUT = 2;
+constexpr uint32_t MAP_CUT = ~0x7fffffffu;
 template <class S> constexpr int WPM = sizeof(S) == 4 ? 1 : 4;         // words of a map
 __device__ inline void publish_map(uint64_t* w, int64_t, float A, float H, uint32_t cut) {
-    uint32_t a = __float_as_uint(A) | 1u;
-    if ((a & 0x7ffffffeu) == 0) a = 3u;
-    if ((__float_as_uint(A) & 0x7fffffffu) == 0x7f800000u) a = (__float_as_uint(A) & 0x80000000u) | 0x7f7fffffu;
-    put(w, (uint64_t(__float_as_uint(H)) << 32) | (cut ? 1u : a));
+    const uint32_t a = A != A ? 0x7fc00000u : __float_as_uint(A);
+    put(w, (uint64_t(__float_as_uint(H)) << 32) | (cut ? MAP_CUT : ~a));
 }
 __device__ inline void publish_map(uint64_t* w, int64_t cw, double A, double H, uint32_t cut) { publish(w, cw, A, cut ? TAG_CUT : TAG_VALUE); publish(w + 2 * cw, cw, H, TAG_VALUE); }
 // `seen`: the first look at the word, taken earlier so that several are on their way together (64 bits: none)
 __device__ inline uint32_t await_map(const uint64_t* w, int64_t, uint64_t seen, float& A, float& H) {
     uint64_t q = seen;
-    while (!(q & 1u)) { __builtin_amdgcn_s_sleep(1); q = get(w); }
-    A = __uint_as_float((uint32_t)q); H = __uint_as_float((uint32_t)(q >> 32));
-    return (uint32_t)q == 1u;
+    while (!(uint32_t)q) { __builtin_amdgcn_s_sleep(1); q = get(w); }
+    A = __uint_as_float(~(uint32_t)q); H = __uint_as_float((uint32_t)(q >> 32));
+    return (uint32_t)q == MAP_CUT;
 }
 __device__ inline uint32_t await_map(const uint64_t* w, int64_t cw, uint64_t, double& A, double& H) {
     const uint32_t q = await_value(w, cw, A);
@@ -234,6 +234,11 @@ template <class S, int V> struct Lds {
 // A state of exactly zero leaves H whatever A is: decays above one may have overflowed in A over the rows, and where one of them is not finite itself H says so already (it starts from
 // the same zero).
 template <class S> __device__ inline S through(S A, S H, uint32_t cut, S c) { return cut || c == S(0) ? H : A * c + H; }
+// Over a tile and more the product of the decays may fall below the smallest number.  What it leaves of a finite state is nothing, but an infinite one stays infinite unless a decay is zero
+// itself: such a product is kept as the smallest number there is, which acts as zero on finite states.  `least` is the smallest of its factors.
+template <class S> constexpr S LEAST = sizeof(S) == 4 ? S(1.40129846e-45f) : S(4.94065645841246544e-324);
+template <class S> __device__ inline S product(S A, S least) { return A == S(0) && least > S(0) ? LEAST<S> : A; }
+template <class S> __device__ inline S far_through(S A, S H, uint32_t cut, S c) { return through(A, H, cut, fabs(A) <= LEAST<S> && fabs(c) < S(INFINITY) ? S(0) : c); }
 
 // The state at the start of position `k` of chain `c` (positions are in scan order; the adjoint counts tiles from the end), given the maps of its NW pieces in sh.A / sh.H / sh.cut
 // (piece order is scan order too).  `first`: the state at the chain's start.  Publishes what later tiles of the chain wait for.  Returns with all pieces' waves past a barrier.
@@ -243,17 +248,19 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
     const int g = k / p.GS, base = g * p.GS, before = k - base, ngroups = (p.ntiles + p.GS - 1) / p.GS;
     const bool last = k == p.ntiles - 1, closes = !last && before == p.GS - 1;
     __syncthreads();
-    S A[V], H[V];
+    S A[V], H[V], least[V];
     uint32_t cut = 0;
     if (wave == 0 && !last) {                                 // the tile's own map
 #pragma unroll
-        for (int v = 0; v < V; ++v) { A[v] = S(1); H[v] = S(0); }
+        for (int v = 0; v < V; ++v) { A[v] = least[v] = S(1); H[v] = S(0); }
         for (int w = 0; w < NW; ++w) {
             const uint32_t q = sh.cut[w];
             cut |= q;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { H[v] = through(sh.A[w][ch + v], sh.H[w][ch + v], q, H[v]); A[v] *= sh.A[w][ch + v]; }
+            for (int v = 0; v < V; ++v) { H[v] = through(sh.A[w][ch + v], sh.H[w][ch + v], q, H[v]); A[v] *= sh.A[w][ch + v]; least[v] = fmin(least[v], fabs(sh.A[w][ch + v])); }
         }
+#pragma unroll
+        for (int v = 0; v < V; ++v) A[v] = product(A[v], least[v]);
         if (!closes) {                                        // (only later tiles of the same group read it)
             uint64_t* dst = p.agg + (c * p.ntiles + k) * WM * CW + ch;
 #pragma unroll
@@ -272,7 +279,7 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
         S a[V], h[V];
         uint32_t q = 0;
 #pragma unroll
-        for (int v = 0; v < V; ++v) { a[v] = S(1); h[v] = S(0); }
+        for (int v = 0; v < V; ++v) { a[v] = least[v] = S(1); h[v] = S(0); }
 #pragma unroll
         for (int m = 0; m < MOST_GS / NW; ++m)
             if (m < per && j0 + m < before) {
@@ -281,26 +288,28 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
                 for (int v = 0; v < V; ++v) {
                     S am, hm;
                     qm = await_map(src + m * WM * CW + v, CW, seen[m][v], am, hm);
-                    h[v] = through(am, hm, qm, h[v]); a[v] *= am;
+                    h[v] = far_through(am, hm, qm, h[v]); a[v] *= am; least[v] = fmin(least[v], fabs(am));
                 }
                 q |= qm;
             }
 #pragma unroll
-        for (int v = 0; v < V; ++v) { sh.pA[wave][ch + v] = a[v]; sh.pH[wave][ch + v] = h[v]; }
+        for (int v = 0; v < V; ++v) { sh.pA[wave][ch + v] = product(a[v], least[v]); sh.pH[wave][ch + v] = h[v]; }
         if (lane == 0) sh.pcut[wave] = q;
     }
     S B[V], G[V];
     uint32_t gcut = 0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) { B[v] = S(1); G[v] = S(0); }
+    for (int v = 0; v < V; ++v) { B[v] = least[v] = S(1); G[v] = S(0); }
     if (before > 0) {
         __syncthreads();
         for (int i = 0; i * per < before; ++i) {
             const uint32_t q = sh.pcut[i];
             gcut |= q;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { G[v] = through(sh.pA[i][ch + v], sh.pH[i][ch + v], q, G[v]); B[v] *= sh.pA[i][ch + v]; }
+            for (int v = 0; v < V; ++v) { G[v] = far_through(sh.pA[i][ch + v], sh.pH[i][ch + v], q, G[v]); B[v] *= sh.pA[i][ch + v]; least[v] = fmin(least[v], fabs(sh.pA[i][ch + v])); }
         }
+#pragma unroll
+        for (int v = 0; v < V; ++v) B[v] = product(B[v], least[v]);
     }
     // the state at the group's start: wave 0 waits for it and, in the group's last tile, has the next group's on its way two operations later
     if (g > 0) {
@@ -311,18 +320,18 @@ template <class S, int V> __device__ inline void chain(const Args& p, Lds<S, V>&
             for (int v = 0; v < V; ++v) {
                 S s;
                 await_value(src + v, CW, s);
-                if (closes) publish(dst + v, CW, through(A[v], H[v], cut, through(B[v], G[v], gcut, s)), TAG_VALUE);
+                if (closes) publish(dst + v, CW, far_through(A[v], H[v], cut, far_through(B[v], G[v], gcut, s)), TAG_VALUE);
                 sh.c[ch + v] = s;
             }
         }
         __syncthreads();
 #pragma unroll
-        for (int v = 0; v < V; ++v) carry[v] = through(B[v], G[v], gcut, sh.c[ch + v]);
+        for (int v = 0; v < V; ++v) carry[v] = far_through(B[v], G[v], gcut, sh.c[ch + v]);
     } else {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            carry[v] = through(B[v], G[v], gcut, first[v]);
-            if (wave == 0 && closes) publish(p.car + (c * ngroups + g + 1) * W * CW + ch + v, CW, through(A[v], H[v], cut, carry[v]), TAG_VALUE);
+            carry[v] = far_through(B[v], G[v], gcut, first[v]);
+            if (wave == 0 && closes) publish(p.car + (c * ngroups + g + 1) * W * CW + ch + v, CW, far_through(A[v], H[v], cut, carry[v]), TAG_VALUE);
         }
     }
 }
