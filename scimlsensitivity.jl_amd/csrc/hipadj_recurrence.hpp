@@ -56,23 +56,21 @@ template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 // ---- values -----------------------------------------------------------------------------------------------------------------------------------------------------
 
-// FAST: where x and gate have 16 bits, exp(g) is exp2(g log2 e) with the product rounded: off by |g| 2^-24 of itself, which is nothing where exp(g) is not nothing.  The states that leave
-// in 32 bits stay as exact; only a gradient with respect to a strongly negative gate is less so, and that is rounded to 16 bits.
+// FAST: where x and gate have 16 bits, exp(g) is exp2(g log2 e) with the product rounded: off by |g| 2^-24 of itself.
 //
-// exp in 32 bits: exp2 of g log2(e) with the product's rounding error carried along, so that strong decays keep their digits; beyond +-200 (0 or inf in 32 bits) the argument is
-// cut off, which also keeps the error term finite for a gate of -inf or of its type's lowest value.  NaN stays NaN.
-template <bool FAST> __device__ inline float exp_(float g) {
-    if constexpr (FAST) return __builtin_amdgcn_exp2f(g * 1.44269504f);
-    g = g < -200.f ? -200.f : (g > 200.f ? 200.f : g);
-    const float p = g * 1.44269504f;
-    const float e = fmaf(g, 1.44269504f, -p) + g * 1.92596299e-8f;
-    const float r = __builtin_amdgcn_exp2f(p);
-    return fmaf(r, e * 0.693147181f, r);
+// exp in 32 bits: exp2 of p = g log2(e), times 1 + (g - p ln 2), which makes up for p's rounding and the constant's: strong decays keep their digits.  The difference is no number where p
+// overflows, where exp2 is 0 or infinite: the smaller of NaN and 1 is 1.  NaN stays NaN.  NEG: g <= 0, nothing overflows upwards and the product takes one instruction less.
+template <bool FAST, bool NEG> __device__ inline float exp_(float g) {
+    const float p = g * 1.44269504f, r = __builtin_amdgcn_exp2f(p);
+    if constexpr (FAST) return r;
+    float e = fmaf(p, 1.90465433e-9f, fmaf(-p, 0.693147182f, g));
+    e = fminf(e, 1.f);
+    return NEG ? fmaf(r, e, r) : r * (1.f + e);
 }
-template <bool FAST> __device__ inline double exp_(double g) { return exp(g); }
+template <bool FAST, bool NEG> __device__ inline double exp_(double g) { return exp(g); }
 // exp(g) and 1 - exp(g), the latter without the cancellation at small |g| (Taylor series; the first term left out is below 2e-8 of the value at 0.35, FAST: 5e-8 at 0.25)
 template <bool FAST> __device__ inline void exp_rest(float g, float& a, float& rest) {
-    a = exp_<FAST>(g);
+    a = exp_<FAST, false>(g);
     float s;
     s = FAST ? 1.f / 720.f : fmaf(g, 1.f / 5040.f, 1.f / 720.f);
     s = fmaf(s, g, 1.f / 120.f); s = fmaf(s, g, 1.f / 24.f); s = fmaf(s, g, 1.f / 6.f); s = fmaf(s, g, 0.5f); s = fmaf(s, g, 1.f);
@@ -90,8 +88,8 @@ __device__ inline double neg_abs(double x) { return -fabs(x); }
 // first, with its own relative accuracy, and a as its difference from one, within half a unit of the last place.
 template <int FORM, bool REST, bool FAST, class S> __device__ inline void decay(S g, S& a, S& rest) {
     if constexpr (FORM == 0) { a = g; if constexpr (REST) rest = S(1) - g; }
-    else if constexpr (FORM == 1) { if constexpr (REST) exp_rest<FAST>(g, a, rest); else a = exp_<FAST>(g); }
-    else { const S e = exp_<FAST>(neg_abs(g)), s = e * recip(S(1) + e), l = S(1) - s; a = g >= S(0) ? l : s; if constexpr (REST) rest = g >= S(0) ? s : l; }
+    else if constexpr (FORM == 1) { if constexpr (REST) exp_rest<FAST>(g, a, rest); else a = exp_<FAST, false>(g); }
+    else { const S e = exp_<FAST, true>(neg_abs(g)), s = e * recip(S(1) + e), l = S(1) - s; a = g >= S(0) ? l : s; if constexpr (REST) rest = g >= S(0) ? s : l; }
 }
 
 // ---- published words ----------------------------------------------------------------------------------------------------------------------------------------------
