@@ -56,14 +56,13 @@ template <class T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
 // ---- values -----------------------------------------------------------------------------------------------------------------------------------------------------
 
-// FAST: where x and gate have 16 bits, exp(g) is exp2(g log2 e) with the product rounded: off by |g| 2^-24 of itself.
-//
-// exp in 32 bits: exp2 of p = g log2(e), times 1 + (g - p ln 2), which makes up for p's rounding and the constant's: strong decays keep their digits.  The difference is no number where p
-// overflows, where exp2 is 0 or infinite: the smaller of NaN and 1 is 1.  NaN stays NaN.  NEG: g <= 0, nothing overflows upwards and the product takes one instruction less.
+// exp in 32 bits: exp2 of p = g log2(e), times 1 + (g - p ln 2), which makes up for p's rounding and the constant's: strong decays keep their digits (without it exp(-14) is off by 10 units
+// of its last place).  ln 2 in one number leaves |g| 3e-9, two units at -80, which 16-bit data (FAST) do with; wider ones have it in two.  The difference is no number where p overflows, where
+// exp2 is 0 or infinite: the smaller of NaN and 1 is 1.  NaN stays NaN.  NEG: g <= 0, nothing overflows upwards and the product takes one instruction less.
 template <bool FAST, bool NEG> __device__ inline float exp_(float g) {
     const float p = g * 1.44269504f, r = __builtin_amdgcn_exp2f(p);
-    if constexpr (FAST) return r;
-    float e = fmaf(p, 1.90465433e-9f, fmaf(-p, 0.693147182f, g));
+    float e = fmaf(-p, 0.693147182f, g);
+    if constexpr (!FAST) e = fmaf(p, 1.90465433e-9f, e);
     e = fminf(e, 1.f);
     return NEG ? fmaf(r, e, r) : r * (1.f + e);
 }

@@ -1,5 +1,9 @@
 """Gates far from zero in the gated linear recurrence (`-m gpu`): decays that overflow, that are tiny, and that stand alone because nothing else reaches a row."""
+import numpy as np
 import pytest
+
+import recurrence_oracle as O
+from test_gpu_recurrence import host
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +31,20 @@ def test_an_exponential_that_overflows_is_infinite(sa, torch, dtype):
     finite = sa.recurrence_solve(x, torch.full_like(g, 700.0 if dtype == "float64" else 88.0)[None, None], h0, form="log").h_final
     assert torch.isfinite(finite).all()
 
+
+@pytest.mark.parametrize("form", ["log", "sigmoid"])
+@pytest.mark.parametrize("dtype,gate_dtype", [("float32", "float32"), ("bfloat16", "bfloat16"), ("float16", "float16"), ("bfloat16", "float32")])
+def test_strong_decays_keep_their_digits_in_the_states(sa, torch, dtype, gate_dtype, form):
+    """One row and nothing added: h_final is the decay times the start and dh0 the decay times the last cotangent, in 32 bits also for 16-bit data, each within the 4 units of a decay and
+    the product's half."""
+    g = torch.linspace(-80.0, 0.0, 4001, dtype=torch.float64).to(getattr(torch, gate_dtype)).cuda()
+    x = torch.zeros(1, 1, 4001, dtype=getattr(torch, dtype), device="cuda")
+    h0 = torch.full((1, 4001), 1.5, device="cuda")
+    sol = sa.recurrence_solve(x, g[None, None], h0, form=form)
+    _, dg, d0 = sa.recurrence_adjoint(sol, None, h0)
+    want = 1.5 * O.decay(form, O.LD(host(g)))[0]
+    for got in (sol.h_final, d0):
+        assert np.abs(host(got)[0] / want - 1).max() <= 4.5 * 2.0 ** -23
+    state = h0.clone()
+    sa.gated_recurrence_step(x[0], g[None], state, form=form)
+    assert np.abs(host(state)[0] / want - 1).max() <= 4.5 * 2.0 ** -23
