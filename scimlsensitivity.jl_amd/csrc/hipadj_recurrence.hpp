@@ -506,7 +506,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 }
 
 // ---- adjoint ------------------------------------------------------------------------------------------------------------------------------------------------------
-// Where 1 - a is needed, 16-bit data keep it in registers and a = 1 - (1 - a) is one instruction; wider ones keep a and evaluate the gate again at the end.  16-bit data also leave x and dh
+// Where both a and 1 - a are needed, 16-bit data keep the smaller one in registers, with its own digits, and the larger one is its difference from one, good to half a unit: both are factors
+// of gradients, and 1 - (1 - a) would have none of a's digits left at exp(-17).  Wider data keep a and evaluate the gate again at the end.  16-bit data also leave x and dh
 // as they arrived and make 32-bit values of them each time they are used (`again` hides that they are the same values), and read dh a second time, from L2: then three workgroups share
 // a CU instead of two (80 registers), and the adjoint of 8 x 4096 x 2048 BF16 takes 164 us instead of 180.  (Not for packed rows where 1 - a is kept: 13-29 registers would spill, 64-75 us
 // for 37 ... 512 sequences of 16384 x 1024 F16 against 64-80.)
@@ -537,10 +538,11 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
     if constexpr (PACKED) m = marks_of<TS>(p, t0, win, seqs[wave]);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
     arrived(rg); arrived(rx); arrived(rd);
-    S kept[TS][V], before[TS][V];                             // 1 - a (INVERSE) or a of each row; the state before it, till then its b unless that is made again from x (LATE)
-    constexpr bool INVERSE = KEEP && FORM != 0;               // 1 - a is what is kept (a given decay is kept itself, 1 - a is its difference from one by definition)
-    auto a = [&](int i, int v) -> S { return INVERSE ? S(1) - kept[i][v] : kept[i][v]; };
-    auto rest_of = [&](int i, int v) -> S { return INVERSE ? kept[i][v] : S(1) - kept[i][v]; };      // KEEP
+    S kept[TS][V], before[TS][V];                             // a or (PAIR) the smaller of a and 1 - a of each row; the state before it, till then its b unless that is made again from x (LATE)
+    constexpr bool PAIR = KEEP && FORM != 0;                  // (a given decay is kept itself, 1 - a is its difference from one by definition)
+    bool low[TS][V];                                          // PAIR: a is what is kept: a mask a row in scalar registers
+    auto a = [&](int i, int v) -> S { return PAIR && !low[i][v] ? S(1) - kept[i][v] : kept[i][v]; };
+    auto rest_of = [&](int i, int v) -> S { return PAIR && !low[i][v] ? kept[i][v] : S(1) - kept[i][v]; };      // KEEP
     auto b_of = [&](int i, int v) -> S {
         if constexpr (!LATE) return before[i][v];
         const S x = (S)part<T, V>(rx[i], v);
@@ -571,7 +573,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         for (int v = 0; v < V; ++v) {
             S aa, rest = S(0);
             decay<FORM, REST, FAST, S>((S)part<TG, V>(rg[i], v), aa, rest);
-            kept[i][v] = INVERSE ? rest : aa;
+            low[i][v] = PAIR && aa < S(0.5);
+            kept[i][v] = PAIR && !low[i][v] ? rest : aa;
             if constexpr (!LATE) before[i][v] = rest * (S)part<T, V>(rx[i], v);
         }
     if (rows < TS) {                                          // rows behind the end pass a state on
@@ -579,7 +582,7 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         for (int i = 0; i < TS; ++i) if (i >= rows) {
             rx[i] = 0; rd[i] = 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { kept[i][v] = INVERSE ? S(0) : S(1); if constexpr (!LATE) before[i][v] = S(0); }
+            for (int v = 0; v < V; ++v) { low[i][v] = false; kept[i][v] = PAIR ? S(0) : S(1); if constexpr (!LATE) before[i][v] = S(0); }
         }
     }
     if constexpr (PACKED) if (m.out) {
@@ -670,7 +673,6 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
 #pragma unroll
         for (int i = TS - 1; i >= 0; --i) {
             Pack<T, V> ox; Pack<TG, V> og;
-            S lastG[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const S G = cot(marked, i, v) + R[v], ai = a(i, v);
@@ -682,7 +684,6 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
                 if constexpr (FORM == 2) da *= ai * rest;
                 S dx = COUPLED ? G * rest : G;
                 R[v] = ai * G;
-                lastG[v] = G;
                 if (marked.value && ((m.out >> i) & 1)) { da = S(0); dx = S(0); R[v] = S(0); }
                 ox.v[v] = (T)dx; og.v[v] = (TG)da;
             }
@@ -691,12 +692,6 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
                 if (p.dgate) write<TG, V>(dgr, lg, og);
             }
             dxr -= p.dx_st; dgr -= p.dg_st;
-            // the gradient of a start leaves in the state's type: 1 - (1 - a) would not do for a small a
-            if (INVERSE && (marked.value ? (m.start >> i) & 1 : !PACKED && i == 0 && tile == 0 && wave == 0)) {
-                const Raw<TG, V> g0 = read<TG, V>((const TG*)p.gate + (b * p.g_sb + (t0 + i) * p.g_st + c0), lg);
-#pragma unroll
-                for (int v = 0; v < V; ++v) { S aa, rest; decay<FORM, false, FAST, S>((S)part<TG, V>(g0, v), aa, rest); R[v] = aa * lastG[v]; }
-            }
             if constexpr (marked.value) {
                 if ((m.start >> i) & 1) {
                     const int64_t s = uniform(seqs[wave][i]);
