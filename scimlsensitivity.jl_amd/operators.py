@@ -44,9 +44,13 @@ def _on(name, t, like, dtype=None, shape=None):
     return t
 
 
+def _adjacent(t):
+    return t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1
+
+
 def _rows(t):
     """t with channels next to each other: as it is, or a copy."""
-    return t if t.dim() == 0 or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+    return t if _adjacent(t) else t.contiguous()
 
 
 def _gate_types(torch, x, gate, form):
@@ -105,7 +109,9 @@ def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
     r.gate, r.coupled, r.batch, r.length, r.channels, r.nseq = GATES[form], int(bool(coupled)), batch, length, channels, nseq
     if packed:
         r.offsets, r.offsets_bits = offsets.data_ptr(), 64 if offsets.dtype == torch.int64 else 32
-    h = torch.empty_like(x)
+    h = torch.empty_like(x)                                  # in x's order of batch and time, where its channels lie next to each other (not so for windows that overlap)
+    if not _adjacent(h):
+        h = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     r.x_stride[:], r.gate_stride[:], r.h_stride[:] = _strides(x, packed), _strides(gate, packed), _strides(h, packed)
     L = _lib.load()
     ck, ws = C.c_int64(), C.c_int64()
