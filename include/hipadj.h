@@ -497,7 +497,8 @@ int hipadj_recurrence_step_dev(int32_t device, int32_t dtype, int32_t gate_dtype
  * — the nearest semi-orthogonal matrix up to the factors the coefficients leave (for (3.4445, -4.7750, 2.0315): singular values in 0.7 ... 1.2).  grad, out [batch][rows][cols] of dtype
  * F32, BF16 or F16, momentum the same shape in F32 (NULL: none), column stride 1, rows and matrices strided.  Arithmetic: products of two-term F16 splits (22 bits) accumulated
  * in F32; for BF16 with both sides of at least 256, one F16 term a factor, whose rounding adds about as much as the output's own.  A matrix with a non-finite entry gives NaN.
- * Coefficients within +-32 under which no singular value can pass 6 and no eigenvalue of c1 A + c2 A A 24 (HIPADJ_ERR_UNSUPPORTED otherwise: F16 factors would overflow).  Sides up to
+ * Coefficients within +-32 under which no singular value can pass 5.6 before a step or 6 behind the last, and no eigenvalue of c1 A + c2 A A 24 (HIPADJ_ERR_UNSUPPORTED otherwise:
+ * F16 factors would overflow).  Sides up to
  * 65536 and 32768, up to 65535 matrices.  out may be grad; momentum overlaps neither.  Sides up to 128 need no workspace, others 256-byte aligned. */
 typedef struct {
     uint32_t struct_size;      /* = sizeof(hipadj_orthogonal) */

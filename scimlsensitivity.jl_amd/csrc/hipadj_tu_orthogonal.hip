@@ -148,10 +148,12 @@ template <class T> static void run(const hipadj_orthogonal* o, const Plan& p, co
 }
 
 // How far the coefficients let the iteration grow: X starts with singular values in [0, 1], a step maps a bound s to the largest |c0 x + c1 x^3 + c2 x^5| on [0, s], reached at s or where
-// the derivative vanishes, and B has eigenvalues c1 y + c2 y^2, y <= s^2.  F16 holds 2^13 X up to 8 and 2^11 B up to 32.
+// the derivative vanishes, and B has eigenvalues c1 y + c2 y^2, y <= s^2.  F16 holds 2^13 X up to 8 and 2^11 A, 2^11 B up to 32: an X that goes into another step, where A = X X' is formed, may
+// have singular values up to 5.6 (its square 31.4), the last one up to 6.
 static bool grows(const hipadj_orthogonal* o, double& s, double& big) {
     s = 1.0; big = 0.0;
     for (int k = 0; k < o->steps; ++k) {
+        if (s > 5.6) return true;
         const double c0 = o->coefficients[3 * k], c1 = o->coefficients[3 * k + 1], c2 = o->coefficients[3 * k + 2];
         auto p = [&](double x) { return std::fabs(x * (c0 + x * x * (c1 + x * x * c2))); };
         auto b = [&](double y) { return std::fabs(y * (c1 + y * c2)); };
@@ -178,7 +180,7 @@ static int check(const hipadj_orthogonal* o) {
     for (int i = 0; i < 3 * o->steps; ++i)
         if (!(std::fabs(o->coefficients[i]) <= 32.0)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: coefficients within +-32, got %g", o->coefficients[i]);
     double s, big;
-    if (grows(o, s, big)) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: with these coefficients singular values can grow to %.3g (at most 6) and c1 A + c2 A A to %.3g (at most 24)", s, big);
+    if (grows(o, s, big)) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: with these coefficients singular values can grow to %.3g (at most 5.6 before a step, 6 behind the last) and c1 A + c2 A A to %.3g (at most 24)", s, big);
     if (!std::isfinite(o->beta) || !std::isfinite(o->scale)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "orthogonalized update: beta and scale must be finite");
     if (std::max(o->rows, o->cols) > 65536 || std::min(o->rows, o->cols) > 32768 || o->batch > 65535)
         return ops_fail(HIPADJ_ERR_UNSUPPORTED, "orthogonalized update: at most 65535 matrices with sides of at most 32768 and 65536");
