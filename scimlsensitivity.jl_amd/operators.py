@@ -66,6 +66,14 @@ def _gate_types(torch, x, gate, form):
     return torch.float64 if x.dtype == torch.float64 else torch.float32
 
 
+def _written(torch, name, t):
+    """Before a call writes t in place, outside of what autograd records: refused where that would make a recorded gradient wrong, and counted as a change of t, so that a graph that has
+    saved t says so."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires grad and is written in place, which has no gradient: call under torch.no_grad(), or pass {name}.detach()")
+    torch.autograd.graph.increment_version(t)
+
+
 class RecurrenceSolution:
     """What recurrence_solve returns: h [like x], h_final [rows][channels], and what recurrence_adjoint needs of the forward pass (x, the gate and h0 by
     reference — they must not change before the adjoint — and the states at the checkpoints)."""
@@ -188,7 +196,7 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
 def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=None):
     """One step of running sequences: state[slots[i]] <- a state[slots[i]] + b in place, and h[i] = the new state in x's type.  x, gate [batch][channels]; state
     [nslots][channels] float32 (float64 for float64); slots int32 / int64 [batch] or None (row i has state i).  A slot outside the states (-1) pads the batch: h[i] = 0.
-    Rows with the same slot are consecutive steps of that state in row order.  No gradients: gated_recurrence over one row has them."""
+    Rows with the same slot are consecutive steps of that state in row order.  No gradients: gated_recurrence over one row has them; a state that requires grad is refused in grad mode."""
     torch = _torch()
     if x.dim() != 2:
         raise ValueError(f"x must be [batch][channels], got shape {tuple(x.shape)}")
@@ -204,6 +212,7 @@ def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=No
     elif state.shape[0] < x.shape[0]:
         raise ValueError(f"{x.shape[0]} rows without slots need as many states, got {state.shape[0]}")
     x, gate = _rows(x), _rows(gate)
+    _written(torch, "state", state)
     h = torch.empty_like(x, memory_format=torch.contiguous_format)
     _check(_lib.load().hipadj_recurrence_step_dev(x.device.index, _DTYPES[x.dtype], _DTYPES[gate.dtype], GATES[form], bool(coupled), x.shape[0], x.shape[1], x.data_ptr(), x.stride(0),
                                                   gate.data_ptr(), gate.stride(0), state.data_ptr(), state.stride(0), state.shape[0], _ptr(slots),
@@ -219,7 +228,7 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     (nesterov) or momentum, X = u / (|u| + 1e-7), `steps` times X <- c0 X + c1 A X + c2 A A X with A = X X', and scale X is returned in grad's type.
 
     grad [..., rows, cols] float32, bfloat16 or float16: every matrix of the leading dimensions by itself (heads, layers); row-major or its transpose.
-    coefficients: three numbers, or three for each step.  out: where to write (like grad; grad itself is allowed).  For weights W [out, in] the usual step is
+    coefficients: three numbers, or three for each step.  out: where to write (like grad; grad itself is allowed); neither momentum nor out may require grad in grad mode.  For weights W [out, in] the usual step is
     W -= lr * orthogonalized_update(dW, m, scale=max(1, out / in) ** 0.5)."""
     torch = _torch()
     if not grad.is_cuda:
@@ -276,6 +285,9 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     L = _lib.load()
     ws = C.c_int64()
     _check(L.hipadj_orthogonalized_update_size(C.byref(q), C.byref(ws)))
+    for name, t in (("momentum", momentum), ("out", given_out)):
+        if t is not None:
+            _written(torch, name, t)
     work = torch.empty(ws.value, dtype=torch.uint8, device=grad.device) if ws.value else None
     _check(L.hipadj_orthogonalized_update_dev(C.byref(q), _ptr(g), _ptr(m), _ptr(o), _ptr(work), ws.value, _stream(torch, grad.device)))
     return given_out if given_out is not None else out

@@ -263,7 +263,7 @@ class WideDeviceFunction(DeviceFunction):
         from . import operators
         blocks = self.weight_blocks()
         host = not isinstance(dp, torch.Tensor)
-        g = torch.as_tensor(np_.ascontiguousarray(dp), device=f"cuda:{int(device)}") if host else dp
+        g = torch.as_tensor(np_.ascontiguousarray(dp), device=f"cuda:{int(device)}") if host else dp.detach()
         if tuple(g.shape) != (self.np,):
             raise ValueError(f"dp must have shape ({self.np},), got {tuple(g.shape)}")
         if momentum is not None and (tuple(momentum.shape) != (self.np,) or momentum.dtype != torch.float32 or momentum.device != g.device or not momentum.is_contiguous()):
