@@ -142,6 +142,9 @@ def recurrence_adjoint(sol, dh=None, dh_final=None, *, need=(True, True, True)):
         raise ValueError("the solution was computed with adjoint=False: it has no checkpoints")
     x, gate, packed = sol.x, sol.gate, sol.offsets is not None
     r = HipadjRecurrence.from_buffer_copy(sol._config)
+    r.x_stride[:], r.gate_stride[:] = _strides(x, packed), _strides(gate, packed)      # of the tensors as they are now: hooks on saved tensors may have laid them out anew
+    if packed:
+        r.offsets = sol.offsets.data_ptr()
     if dh is not None:
         dh = _rows(_on("dh", dh, x, x.dtype, x.shape))
         r.dh_stride[:] = _strides(dh, packed)
@@ -176,7 +179,9 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
                 want = any(ctx.needs_input_grad[:3])
                 sol = recurrence_solve(x, gate, h0, form=form, coupled=coupled, offsets=offsets, adjoint=want)
                 if want:
-                    ctx.save_for_backward(sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints)      # versions are checked: a changed input is an error, not a wrong gradient
+                    saved = (sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints)
+                    ctx.save_for_backward(*saved)            # versions are checked: a changed input is an error, not a wrong gradient
+                    ctx.kinds = [(None, None, None) if t is None else (t.dtype, t.shape, t.device) for t in saved]
                     ctx.rest = (sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape)
                     ctx.set_materialize_grads(False)
                 return sol.h, sol.h_final
@@ -185,7 +190,12 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
             @torch.autograd.function.once_differentiable
             def backward(ctx, dh, dh_final):
                 sol = RecurrenceSolution()
-                sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints = ctx.saved_tensors
+                saved = []
+                for name, t, (dtype, shape, device) in zip(("x", "gate", "h0", "offsets", "the checkpoints"), ctx.saved_tensors, ctx.kinds):
+                    if t is not None and (t.dtype, t.shape, t.device) != (dtype, shape, device):
+                        raise ValueError(f"{name} was saved as {dtype} {tuple(shape)} on {device} and came back as {t.dtype} {tuple(t.shape)} on {t.device}")
+                    saved.append(t if t is None else _rows(t) if name in ("x", "gate") else t.contiguous())
+                sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints = saved
                 sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape = ctx.rest
                 dx, dgate, dh0 = recurrence_adjoint(sol, dh, dh_final, need=ctx.needs_input_grad[:3])
                 return dx, dgate, dh0, None, None, None

@@ -61,3 +61,33 @@ def test_the_step_of_a_chain_takes_a_gradient_that_requires_grad(sa, torch):
     dp = torch.randn(fun.np, device="cuda", generator=torch.Generator("cuda").manual_seed(2))
     got = fun.orthogonalized_update(dp.clone().requires_grad_())
     assert not got.requires_grad and torch.equal(got, fun.orthogonalized_update(dp))
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_saved_tensors_that_come_back_in_another_layout(sa, torch, packed):
+    """Hooks that move saved tensors to the host and back, or hand out copies with other strides: slices and broadcast gates come back dense, offsets at another address."""
+    both = rows(torch, 2, 90, 24).requires_grad_()
+    gate = rows(torch, 12).requires_grad_()
+    h0 = rows(torch, 4 if packed else 2, 12).requires_grad_()
+    off = torch.tensor([0, 20, 20, 61, 85], dtype=torch.int32, device="cuda")
+    dh = rows(torch, 2, 90, 12)
+
+    def grads(broadcast):
+        x, g = both[..., :12], (-gate.abs()).expand(2, 90, 12) if broadcast else -both[..., 12:].abs()
+        kw, d = {}, dh
+        if packed:
+            x, g, d, kw = x[0], g[0], dh[0], dict(offsets=off.clone())
+        h, last = sa.gated_recurrence(x, g, h0, coupled=True, **kw)
+        kw.clear()
+        torch.full((5,), 1 << 20, dtype=torch.int32, device="cuda")          # what a freed copy of the offsets would hold
+        return torch.autograd.grad((h * d).sum() + last.sum(), [both, gate, h0] if broadcast else [both, h0])
+    for broadcast in (False, True):
+        want = grads(broadcast)
+        with torch.autograd.graph.save_on_cpu():
+            assert all(torch.equal(a, b) for a, b in zip(grads(broadcast), want))
+        for pack, unpack in ((lambda t: t, lambda t: t.clone(memory_format=torch.contiguous_format)), (lambda t: t, lambda t: t.t().contiguous().t() if t.dim() == 2 else t)):
+            with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+                assert all(torch.equal(a, b) for a, b in zip(grads(broadcast), want))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.double() if t.is_floating_point() else t), pytest.raises(ValueError, match="came back as"):
+        h, _ = sa.gated_recurrence(rows(torch, 1, 9, 4).requires_grad_(), -rows(torch, 1, 9, 4).abs())
+        h.sum().backward()
