@@ -230,6 +230,20 @@ def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=No
     return h
 
 
+def _disjoint(t):
+    """Whether no two elements of t [batch, rows, cols] share a place, for a t with columns or rows next to each other (others are refused for that)."""
+    if t.numel() == 0:
+        return True
+    t = t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.transpose(-1, -2)
+    (batch, rows, cols), (sb, sr, _) = t.shape, t.stride()
+    if rows > 1 and sr < cols:
+        return False
+    if batch == 1 or sb > (rows - 1) * sr + cols - 1 or (sb >= cols and sr > (batch - 1) * sb + cols - 1):      # one behind the other, or side by side
+        return True
+    # matrix k starts k sb behind the first: not within cols of one of its rows
+    return all(k * sb - r * sr >= cols and (r + 1 >= rows or (r + 1) * sr - k * sb >= cols) for k in range(1, batch) for r in (min(rows - 1, k * sb // max(sr, 1)),))
+
+
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)      # the usual quintic: steep at zero, singular values end in 0.7 ... 1.2 (K. Jordan, Muon, 2024)
 
 
@@ -262,9 +276,6 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
         except RuntimeError:
             return None
 
-    def own(t):            # written in place: no two elements in one place
-        return t.numel() == 0 or all(s > 0 or n == 1 for s, n in zip(t.stride(), t.shape))
-
     given_out = out
     if out is None:
         out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if grad.stride(-1) == 1 or grad.stride(-2) != 1 else \
@@ -272,7 +283,7 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     g, m, o = matrices(grad), None if momentum is None else matrices(momentum), matrices(out)
     if g is None:
         g = matrices(grad.contiguous())
-    if (momentum is not None and (m is None or not own(m))) or o is None or not own(o):
+    if (momentum is not None and (m is None or not _disjoint(m))) or o is None or not _disjoint(o):
         raise ValueError("momentum and out are written in place: their matrices must lie at one stride from each other and not overlap")
     # one order for all: columns next to each other, or the transposes (the iteration commutes with transposition)
     row_major = lambda t: t.shape[-1] <= 1 or t.stride(-1) == 1       # noqa: E731
