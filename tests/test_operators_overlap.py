@@ -32,4 +32,4 @@ def test_overlapping_rows_are_refused(sa):
             with pytest.raises(ValueError, match="not overlap"):
                 sa.orthogonalized_update(g, **kw)
     heads = z(5, 2, 4).transpose(0, 1)                                         # matrices side by side
-    assert sa.orthogonalized_update(g, out=heads) is heads and sa.orthogonalized_update(g, z(2, 4, 5).transpose(1, 2)).shape == g.shape
+    assert sa.orthogonalized_update(g, out=heads) is heads and sa.orthogonalized_update(z(2, 4, 5).transpose(1, 2), z(2, 4, 5).transpose(1, 2)).shape == g.shape
