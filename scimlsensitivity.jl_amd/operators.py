@@ -77,7 +77,7 @@ def _written(torch, name, t):
 class RecurrenceSolution:
     """What recurrence_solve returns: h [like x], h_final [rows][channels], and what recurrence_adjoint needs of the forward pass (x, the gate and h0 by
     reference — they must not change before the adjoint — and the states at the checkpoints)."""
-    __slots__ = ("h", "h_final", "x", "gate", "h0", "offsets", "form", "coupled", "_checkpoints", "_config", "_workspace_bytes", "_state_type", "_final_shape")
+    __slots__ = ("h", "h_final", "x", "gate", "h0", "offsets", "form", "coupled", "_checkpoints", "_config", "_workspace_bytes", "_state_type", "_final_shape", "_stream")
 
 
 def _strides(t, packed):
@@ -128,7 +128,8 @@ def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
     sol.h, sol.h_final = h, torch.empty((rows, channels), dtype=wide, device=x.device)
     sol._checkpoints = torch.empty(ck.value, dtype=torch.uint8, device=x.device) if adjoint else None
     work = torch.empty(ws.value, dtype=torch.uint8, device=x.device) if ws.value else None
-    _check(L.hipadj_recurrence_forward_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(h0), _ptr(h), _ptr(sol.h_final), _ptr(sol._checkpoints), _ptr(work), ws.value, _stream(torch, x.device)))
+    sol._stream = _stream(torch, x.device)
+    _check(L.hipadj_recurrence_forward_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(h0), _ptr(h), _ptr(sol.h_final), _ptr(sol._checkpoints), _ptr(work), ws.value, sol._stream))
     sol.x, sol.gate, sol.h0, sol.offsets, sol.form, sol.coupled = x, gate, h0, offsets, form, bool(coupled)
     sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape = r, ws.value, wide, (rows, channels)
     return sol
@@ -136,7 +137,8 @@ def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
 
 def recurrence_adjoint(sol, dh=None, dh_final=None, *, need=(True, True, True)):
     """(dx, dgate, dh0): the gradients of sum(dh * h) + sum(dh_final * h_final) with respect to x, gate and h0 (also for h0=None: of the zeros), each of its
-    argument's type; dh [like h], dh_final [like h_final], None = zeros.  need: which of the three to compute (the others are None)."""
+    argument's type; dh [like h], dh_final [like h_final], None = zeros.  need: which of the three to compute (the others are None).  On a stream other than the solution's, that stream
+    has to wait for the solution's first, as for any tensor."""
     torch = _torch()
     if sol._checkpoints is None:
         raise ValueError("the solution was computed with adjoint=False: it has no checkpoints")
@@ -157,9 +159,14 @@ def recurrence_adjoint(sol, dh=None, dh_final=None, *, need=(True, True, True)):
         r.dx_stride[:] = _strides(dx, packed)
     if dgate is not None:
         r.dgate_stride[:] = _strides(dgate, packed)
+    stream = _stream(torch, x.device)
+    if stream != sol._stream:                                # what the solution holds of its own is not to be handed out again before this stream has read it
+        for t in (x, gate, sol.h0, sol.offsets, sol._checkpoints):
+            if t is not None:
+                t.record_stream(torch.cuda.current_stream(x.device))
     work = torch.empty(sol._workspace_bytes, dtype=torch.uint8, device=x.device) if sol._workspace_bytes else None
     _check(_lib.load().hipadj_recurrence_adjoint_dev(C.byref(r), _ptr(x), _ptr(gate), _ptr(sol.h0), _ptr(sol._checkpoints), _ptr(dh), _ptr(dh_final), _ptr(dx), _ptr(dgate), _ptr(dh0),
-                                                     _ptr(work), sol._workspace_bytes, _stream(torch, x.device)))
+                                                     _ptr(work), sol._workspace_bytes, stream))
     return dx, dgate, dh0
 
 
@@ -182,7 +189,7 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
                     saved = (sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints)
                     ctx.save_for_backward(*saved)            # versions are checked: a changed input is an error, not a wrong gradient
                     ctx.kinds = [(None, None, None) if t is None else (t.dtype, t.shape, t.device) for t in saved]
-                    ctx.rest = (sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape)
+                    ctx.rest = (sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape, sol._stream)
                     ctx.set_materialize_grads(False)
                 return sol.h, sol.h_final
 
@@ -196,7 +203,7 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
                         raise ValueError(f"{name} was saved as {dtype} {tuple(shape)} on {device} and came back as {t.dtype} {tuple(t.shape)} on {t.device}")
                     saved.append(t if t is None else _rows(t) if name in ("x", "gate") else t.contiguous())
                 sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints = saved
-                sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape = ctx.rest
+                sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape, sol._stream = ctx.rest
                 dx, dgate, dh0 = recurrence_adjoint(sol, dh, dh_final, need=ctx.needs_input_grad[:3])
                 return dx, dgate, dh0, None, None, None
         _function = GatedRecurrence
