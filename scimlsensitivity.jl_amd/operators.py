@@ -182,8 +182,8 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
     if _function is None:
         class GatedRecurrence(torch.autograd.Function):
             @staticmethod
-            def forward(ctx, x, gate, h0, form, coupled, offsets):
-                want = any(ctx.needs_input_grad[:3])
+            def forward(ctx, x, gate, h0, form, coupled, offsets, graph):
+                want = graph and any(ctx.needs_input_grad[:3])      # (the latter are set under no_grad too)
                 sol = recurrence_solve(x, gate, h0, form=form, coupled=coupled, offsets=offsets, adjoint=want)
                 if want:
                     saved = (sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints)
@@ -205,9 +205,9 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
                 sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints = saved
                 sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape, sol._stream = ctx.rest
                 dx, dgate, dh0 = recurrence_adjoint(sol, dh, dh_final, need=ctx.needs_input_grad[:3])
-                return dx, dgate, dh0, None, None, None
+                return dx, dgate, dh0, None, None, None, None
         _function = GatedRecurrence
-    return _function.apply(x, gate, h0, form, coupled, offsets)
+    return _function.apply(x, gate, h0, form, coupled, offsets, torch.is_grad_enabled())
 
 
 def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=None):

@@ -91,3 +91,18 @@ def test_saved_tensors_that_come_back_in_another_layout(sa, torch, packed):
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t.double() if t.is_floating_point() else t), pytest.raises(ValueError, match="came back as"):
         h, _ = sa.gated_recurrence(rows(torch, 1, 9, 4).requires_grad_(), -rows(torch, 1, 9, 4).abs())
         h.sum().backward()
+
+
+def test_no_checkpoints_where_no_gradient_can_follow(sa, torch, monkeypatch):
+    """Parameters require grad, but not under no_grad: only the forward pass's own bytes are written."""
+    from scimlsensitivity_jl_amd import operators
+    asked, solve = [], operators.recurrence_solve
+    monkeypatch.setattr(operators, "recurrence_solve", lambda *a, **kw: (asked.append(kw["adjoint"]), solve(*a, **kw))[1])
+    x = rows(torch, 2, 200, 8).requires_grad_()
+    h, _ = operators.gated_recurrence(x, -x.abs())
+    with torch.no_grad():
+        again, _ = operators.gated_recurrence(x, -x.abs())
+    with torch.inference_mode():
+        operators.gated_recurrence(x, -x.abs())
+    operators.gated_recurrence(x.detach(), -x.detach().abs())
+    assert asked == [True, False, False, False] and torch.equal(h, again) and h.requires_grad and not again.requires_grad
