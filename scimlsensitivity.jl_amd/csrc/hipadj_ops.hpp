@@ -2,6 +2,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 #include <cstdio>
+#include <tuple>
 #include "../../include/hipadj.h"
 
 void ops_set_error(const char* text);          // hipadj_api.hip: the text of hipadj_last_error(NULL), per thread
@@ -14,11 +15,22 @@ template <class... A> static int ops_fail(int code, const char* format, A... arg
 }
 static inline int ops_fail(int code, const char* text) { ops_set_error(text); return code; }
 
+// A launch whose status is the launch's own: what hipGetLastError holds may be an earlier error of the host program, which stays there for the program to see.
+inline thread_local hipError_t ops_status = hipSuccess;                 // first failure of the current call's launches
+template <class... P, class... A> static void ops_launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t stream, const A&... a) {
+    std::tuple<P...> p(a...);
+    std::apply([&](P&... q) {
+        void* args[] = {(void*)&q...};
+        const hipError_t e = hipLaunchKernel((const void*)kernel, grid, block, args, 0, stream);
+        if (ops_status == hipSuccess) ops_status = e;
+    }, p);
+}
+
 // makes `device` current for the duration of a call and the caller's device current again afterwards
 struct OpsDevice {
     int rc = HIPADJ_OK, old = -1;
     explicit OpsDevice(int device) {
-        (void)hipGetLastError();                    // of an earlier call of the host program: ops_launched reports this call's launches
+        ops_status = hipSuccess;
         int n = 0;
         if (hipGetDeviceCount(&n) != hipSuccess || n <= 0) { (void)hipGetLastError(); rc = ops_fail(HIPADJ_ERR_NO_DEVICE, "no usable HIP device (gfx950 required; there is no CPU fallback)"); return; }
         if (device < 0 || device >= n) { rc = ops_fail(HIPADJ_ERR_INVALID_ARG, "device %d out of range (%d visible)", device, n); return; }
@@ -34,6 +46,7 @@ struct OpsDevice {
 
 // a refused launch (bad grid, no code object for the device) is a status of the call that made it
 static inline int ops_launched(const char* what) {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? HIPADJ_OK : ops_fail(HIPADJ_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+    if (ops_status == hipSuccess) return HIPADJ_OK;
+    (void)hipGetLastError();                        // this call reports it
+    return ops_fail(HIPADJ_ERR_HIP, "%s: %s", what, hipGetErrorString(ops_status));
 }

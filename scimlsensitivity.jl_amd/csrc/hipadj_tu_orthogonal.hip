@@ -49,7 +49,7 @@ static int64_t tiles_of(const Product& g, int64_t batch, bool lower, int64_t BT)
 }
 template <class T, int BT, int EPI, bool SPLIT, int SLOTS> static void product(const Product& g, const Mat& q, const Io<T>& io, int from, int to, hipStream_t s) {
     const dim3 grid((uint32_t)(tiles_of(g, 1, EPI != APPLY && EPI != LAST, BT) * (EPI == PARTS ? g.parts : 1)), 1, (uint32_t)q.batch);
-    k_product<T, BT, EPI, SPLIT, SLOTS><<<grid, dim3(256), 0, s>>>(g, q, io, from, to);
+    ops_launch(k_product<T, BT, EPI, SPLIT, SLOTS>, grid, dim3(256), s, g, q, io, from, to);
 }
 
 // The time of a product by tiles of BT, microseconds: rounds over the 256 CUs, each with a fixed part (first requests, epilogue) and one for every row of K, which grows with the share
@@ -100,10 +100,10 @@ template <class T, bool SPLIT> static void iterate(const hipadj_orthogonal* o, c
     const int64_t rows = flat ? 1 : io.rows, cols = flat ? io.rows * io.cols : io.cols;
     auto aligned = [&](const void* p, int64_t sb, int64_t sr, int64_t per) { return (uintptr_t)p % 16 == 0 && (q.batch == 1 || sb % per == 0) && (rows == 1 || sr % per == 0); };
     const bool vec = cols % 8 == 0 && aligned(io.grad, io.g_b, io.g_r, 16 / sizeof(T)) && (!io.mom || aligned(io.mom, io.m_b, io.m_r, 4));
-    k_norm<T><<<dim3((uint32_t)q.nblocks, (uint32_t)q.batch), dim3(256), 0, s>>>(io, rows, cols, vec, q.partial);
+    ops_launch(k_norm<T>, dim3((uint32_t)q.nblocks, (uint32_t)q.batch), dim3(256), s, io, rows, cols, vec, q.partial);
     const dim3 pieces((uint32_t)(q.np / 64), (uint32_t)(q.mp / 64), (uint32_t)q.batch);
-    if (q.np / 64 * (q.mp / 64) * q.batch <= 1024) k_start<T, SPLIT, 16><<<pieces, dim3(1024), 0, s>>>(io, q);
-    else k_start<T, SPLIT, 4><<<pieces, dim3(256), 0, s>>>(io, q);
+    if (q.np / 64 * (q.mp / 64) * q.batch <= 1024) ops_launch(k_start<T, SPLIT, 16>, pieces, dim3(1024), s, io, q);
+    else ops_launch(k_start<T, SPLIT, 4>, pieces, dim3(256), s, io, q);
     const int64_t smm = q.mp * q.mp, smn = q.mp * q.np;
     auto rounded = [&](int step) { return !SPLIT && step >= o->steps - 2; };
     for (int step = 0; step < o->steps; ++step) {
@@ -138,9 +138,9 @@ template <class T> static void run(const hipadj_orthogonal* o, const Plan& p, co
         Coefficients co;
         for (int i = 0; i < 3 * o->steps; ++i) co.c[i] = (float)o->coefficients[i];
         const dim3 grid((uint32_t)o->batch);
-        if (p.q.n <= 32) k_small<T, 32><<<grid, dim3(64), 0, s>>>(io, p.q.m, p.q.n, p.q.flip, o->steps, co);
-        else if (p.q.n <= 64) k_small<T, 64><<<grid, dim3(256), 0, s>>>(io, p.q.m, p.q.n, p.q.flip, o->steps, co);
-        else k_small<T, 128><<<grid, dim3(1024), 0, s>>>(io, p.q.m, p.q.n, p.q.flip, o->steps, co);
+        if (p.q.n <= 32) ops_launch(k_small<T, 32>, grid, dim3(64), s, io, p.q.m, p.q.n, p.q.flip, o->steps, co);
+        else if (p.q.n <= 64) ops_launch(k_small<T, 64>, grid, dim3(256), s, io, p.q.m, p.q.n, p.q.flip, o->steps, co);
+        else ops_launch(k_small<T, 128>, grid, dim3(1024), s, io, p.q.m, p.q.n, p.q.flip, o->steps, co);
         return;
     }
     if (p.split) iterate<T, true>(o, p.q, io, s);

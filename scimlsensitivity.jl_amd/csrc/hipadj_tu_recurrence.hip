@@ -1,5 +1,6 @@
 // hipadj_tu_recurrence.hip — translation units of the gated linear recurrence: hipcc -DHIPADJ_TU_PAIR=<rec::PAIR_*>; without it the C entry points.
 #include <algorithm>
+#include "hipadj_ops.hpp"
 #include "hipadj_recurrence.hpp"
 
 #if defined(HIPADJ_TU_PAIR)
@@ -9,11 +10,11 @@ template <int PAIR, int V, int FORM, bool COUPLED> static void pick(const Args& 
     typedef Types<PAIR> Y;
     const dim3 grid((uint32_t)((int64_t)a.nchains * a.ntiles)), block(NT);
     if (adjoint) {
-        if (packed) k_adjoint<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, true><<<grid, block, 0, s>>>(a);
-        else k_adjoint<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, false><<<grid, block, 0, s>>>(a);
+        if (packed) ops_launch(k_adjoint<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, true>, grid, block, s, a);
+        else ops_launch(k_adjoint<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, false>, grid, block, s, a);
     } else {
-        if (packed) k_forward<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, true><<<grid, block, 0, s>>>(a);
-        else k_forward<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, false><<<grid, block, 0, s>>>(a);
+        if (packed) ops_launch(k_forward<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, true>, grid, block, s, a);
+        else ops_launch(k_forward<typename Y::T, typename Y::TG, typename Y::S, V, FORM, COUPLED, false>, grid, block, s, a);
     }
 }
 template <int PAIR, int V> static void pick_form(const Args& a, bool adjoint, int form, bool coupled, bool packed, hipStream_t s) {
@@ -31,8 +32,8 @@ template <int PAIR, int V, int FORM> static void pick_step(const StepArgs& a, bo
     typedef Types<PAIR> Y;
     const int ncg = (int)((a.D + NS * V - 1) / (NS * V));
     const dim3 grid((uint32_t)(a.B * ncg)), block(NS);
-    if (coupled) k_step<typename Y::T, typename Y::TG, typename Y::S, V, FORM, true><<<grid, block, 0, s>>>(a, ncg);
-    else k_step<typename Y::T, typename Y::TG, typename Y::S, V, FORM, false><<<grid, block, 0, s>>>(a, ncg);
+    if (coupled) ops_launch(k_step<typename Y::T, typename Y::TG, typename Y::S, V, FORM, true>, grid, block, s, a, ncg);
+    else ops_launch(k_step<typename Y::T, typename Y::TG, typename Y::S, V, FORM, false>, grid, block, s, a, ncg);
 }
 template <int PAIR, int V> static void pick_step_form(const StepArgs& a, int form, bool coupled, hipStream_t s) {
     if (form == 0) pick_step<PAIR, V, 0>(a, coupled, s); else if (form == 1) pick_step<PAIR, V, 1>(a, coupled, s); else pick_step<PAIR, V, 2>(a, coupled, s);
@@ -46,8 +47,6 @@ template void launch_step<HIPADJ_TU_PAIR>(const StepArgs&, bool, int, bool, hipS
 }  // namespace rec
 #else
 #include <cstdio>
-#include "../../include/hipadj.h"
-#include "hipadj_ops.hpp"
 
 namespace rec {
 
@@ -135,8 +134,8 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
         void* to = adjoint ? a.dh0 : a.h_final;
         const void* from = adjoint ? a.dh_final : a.h0;
         const dim3 grid((uint32_t)std::min<int64_t>(1024, (n + 255) / 256)), block(256);
-        if (to && r->dtype == HIPADJ_F64) k_same<double><<<grid, block, 0, (hipStream_t)stream>>>((double*)to, (const double*)from, n);
-        else if (to) k_same<float><<<grid, block, 0, (hipStream_t)stream>>>((float*)to, (const float*)from, n);
+        if (to && r->dtype == HIPADJ_F64) ops_launch(k_same<double>, grid, block, (hipStream_t)stream, (double*)to, (const double*)from, n);
+        else if (to) ops_launch(k_same<float>, grid, block, (hipStream_t)stream, (float*)to, (const float*)from, n);
         return ops_launched("recurrence");
     }
     if (words) {
@@ -145,7 +144,7 @@ static int go(const hipadj_recurrence* r, Args& a, bool adjoint, void* workspace
         uint64_t* w = (uint64_t*)workspace;
         const int64_t W = r->dtype == HIPADJ_F64 ? WPM<double> : WPM<float>;
         a.ticket = (uint32_t*)w; a.agg = w + 1; a.car = a.agg + (int64_t)a.nchains * a.ntiles * W * 64 * V;
-        k_zero<<<dim3((uint32_t)std::min<int64_t>(1024, (words + 255) / 256)), dim3(256), 0, (hipStream_t)stream>>>(w, words);
+        ops_launch(k_zero, dim3((uint32_t)std::min<int64_t>(1024, (words + 255) / 256)), dim3(256), (hipStream_t)stream, w, words);
     }
     run(pair, a, adjoint, wide, r->gate, r->coupled != 0, r->nseq > 0, (hipStream_t)stream);
     return ops_launched("recurrence");
