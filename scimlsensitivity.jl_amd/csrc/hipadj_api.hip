@@ -1992,12 +1992,12 @@ static int stage_down_finish(hipadj_handle* h, double* dst, const double* pin, s
 // The staging block lives in its OWN anonymous mapping with an inaccessible guard page on either side — never in the brk heap.  Round 5's block was posix_memalign memory: once
 // glibc's dynamic mmap threshold has risen (a larger block was freed earlier), such a block comes from the heap, page-adjacent to the caller's small arrays, and registering it
 // there made the next pageable device-to-host copy into a fresh heap array just below it die with "Memory access fault by GPU ... Write access to a read-only page" (the one-in-
-// a-dozen abort of round 5's bench; reproduced in seconds by scripts/r6/fault_stress.py, reduced in scripts/r6/repro_readonly_fault.hip; profiles/r6_fault_*).  The guard pages
+// a-dozen abort of the bench; profiles/r6_fault_*).  The guard pages
 // keep the kernel from merging the mapping with a neighbour's and the registration from sharing a page with anything else.
 static void host_pin_release(hipadj_handle* h) {
     if (!h->h_pin) return;
     (void)hipHostUnregister(h->h_pin);
-    if (h->pin_map_len) (void)munmap((char*)h->h_pin - 4096, h->pin_map_len); else std::free(h->h_pin);      // (else: the reproduction hook's heap block)
+    (void)munmap((char*)h->h_pin - 4096, h->pin_map_len);
     h->h_pin = nullptr; h->pin_count = 0; h->pin_map_len = 0;
 }
 static double* host_pin(hipadj_handle* h, size_t count) {      // the handle's pinned block, grown on demand; nullptr: no pinned memory to be had (the pageable copy still works)
@@ -2007,15 +2007,6 @@ static double* host_pin(hipadj_handle* h, size_t count) {      // the handle's p
     // ordinary (cached) pages, registered with the runtime: hipHostMalloc's default block is fine-grained coherent memory, which the host WRITES at a fraction of its memcpy rate
     // (measured: the staged upload took 12.5 ms against 7.7 ms for the plain pageable copy, profiles/r5_visit2_bench.json)
     const size_t bytes = count * sizeof(double), len = (bytes + 4095) / 4096 * 4096 + 2 * 4096;
-    if (std::getenv("HIPADJ_PIN_HEAP")) {      // REPRODUCTION HOOK (scripts/r6/fault_ab.py): round 5's block, posix_memalign memory registered in place — never use otherwise
-        void* q = nullptr;
-        if (posix_memalign(&q, 4096, bytes) != 0 || !q) return nullptr;
-        std::memset(q, 0, bytes);
-        if (hipHostRegister(q, bytes, hipHostRegisterDefault) != hipSuccess) { (void)hipGetLastError(); std::free(q); return nullptr; }
-        h->h_pin = (double*)q; h->pin_count = count; h->pin_map_len = 0;
-        if (std::getenv("HIPADJ_TRACE_PIN")) std::fprintf(stderr, "hipadj host_pin: handle %p registered [%p, %p) (HEAP block: reproduction hook)\n", (void*)h, q, (void*)((char*)q + bytes));
-        return h->h_pin;
-    }
     char* m = (char*)mmap(nullptr, len, PROT_READ | PROT_WRITE, MAP_PRIVATE | MAP_ANONYMOUS, -1, 0);
     if (m == (char*)MAP_FAILED) return nullptr;
     (void)mprotect(m, 4096, PROT_NONE); (void)mprotect(m + len - 4096, 4096, PROT_NONE);
@@ -2030,8 +2021,8 @@ static double* host_pin(hipadj_handle* h, size_t count) {      // the handle's p
 // EVERY transfer between a caller's host array and the device goes through the handle's staging block (round 6): the host side of each DMA is memory this library owns,
 // registered once, in its own mapping — the caller's arrays are only ever touched by the CPU.  Why: a pageable hipMemcpy makes the runtime pin the caller's pages on the fly and
 // keep those pins cached; with the arrays of a numpy / Julia host (allocated, freed and re-allocated at the same heap addresses from call to call) a device-to-host copy of du0
-// ended in "Memory access fault by GPU ... Write access to a read-only page" and took the host process with it (round 5: one bench run in a dozen; round 6: reproduced in the
-// first seconds of scripts/r6/fault_stress.py, profiles/r6_fault_stress_reproduced_visit3.log; A/B of the three transfer modes: scripts/r6/fault_ab.py).  Staging costs one
+// ended in "Memory access fault by GPU ... Write access to a read-only page" and took the host process with it (round 5: one bench run in a dozen; round 6: found in a stress run,
+// profiles/r6_fault_stress_reproduced_visit3.log; A/B of the three transfer modes: profiles/r6_fault_ab_three_transfer_modes.jsonl).  Staging costs one
 // CPU copy per block (host_copy_par: a few threads at memcpy rate — 24 MB of out / Delta in ~0.5 ms) and removes the runtime's on-the-fly pinning from the path altogether.
 // HIPADJ_HOST_DIRECT=1 restores the direct pageable copies (A/B); HIPADJ_NO_PINNED=1 or a failed registration fall back to them as well.
 static bool host_direct() { static const bool v = [] { const char* e = std::getenv("HIPADJ_HOST_DIRECT"); return e && e[0] == '1'; }(); return v; }

@@ -1,6 +1,6 @@
 #!/bin/bash
 # round 6, visit 2: the GPU suite on four xdist workers (wall time), the wave timeline of a 1250-trajectory shard (trace builds: kernarg-inline vs global segment bounds), the shard sizes
-# with both libraries, then the hunt for round 5's memory fault (consecutive default bench runs)
+# with both libraries
 O=gpurun_out/r6
 mkdir -p $O
 ( time timeout 1100 python -m pytest tests -x -q -m gpu -p no:cacheprovider ) > $O/v2_gpu_suite_xdist.log 2>&1
@@ -13,4 +13,3 @@ timeout 200 python scripts/r6/shard_time.py inline_bounds > $O/v2_shard_time.jso
 HIPADJ_LIBRARY=$PWD/scripts/r6/libhipadj_gb.so timeout 200 python scripts/r6/shard_time.py global_bounds >> $O/v2_shard_time.jsonl 2>> $O/v2_shard_time.err
 timeout 200 python scripts/r6/shard_time.py inline_bounds_again 1250 2500 >> $O/v2_shard_time.jsonl 2>> $O/v2_shard_time.err
 cat $O/v2_shard_time.jsonl | cut -c1-200
-bash scripts/r6/fault_hunt.sh ${HUNT_RUNS:-40}

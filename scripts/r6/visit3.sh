@@ -1,6 +1,6 @@
 #!/bin/bash
 # round 6, visit 3: the library-side dense-chain route and the grouped one-launch pass (tests), the wave timeline with hardware ids, the top segment's weight (HIPADJ_WTOP) at the
-# shard and at the headline size, the grouped form (G waves per workgroup, LDS first level) against the plain one, then the targeted fault stress
+# shard and at the headline size, the grouped form (G waves per workgroup, LDS first level) against the plain one
 O=gpurun_out/r6
 mkdir -p $O
 timeout 600 python -m pytest tests/test_gpu_wide.py tests/test_gpu_fused.py tests/test_gpu_device_loss.py -q -m gpu -p no:cacheprovider -k "routed or dense_chain or grouped or loss_value or virtual" > $O/v3_tests.log 2>&1
@@ -24,5 +24,3 @@ run plain 10000 0 0 4; run g4_12_r4 10000 4 12 4; run g4_8_r4 10000 4 8 4; run g
 cut -c1-170 $O/v3_group.jsonl
 HIPADJ_LIBRARY=$T HIPADJ_FUSED_GROUP=8 HIPADJ_TREE_RADIX=16 timeout 200 python scripts/r6/wave_trace.py 1250 96 > $O/v3_wave_1250_g8.jsonl 2>> $O/v3_wave.err
 HIPADJ_LIBRARY=$T HIPADJ_FUSED_GROUP=4 HIPADJ_TREE_RADIX=16 timeout 200 python scripts/r6/wave_trace.py 1250 48 > $O/v3_wave_1250_g4.jsonl 2>> $O/v3_wave.err
-HIPADJ_TRACE_PIN=1 timeout 900 python scripts/r6/fault_stress.py 3 > $O/v3_stress.json 2> $O/v3_stress.err
-echo "stress rc=$?"; cat $O/v3_stress.json; tail -n 2 $O/v3_stress.err

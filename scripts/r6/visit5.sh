@@ -1,12 +1,8 @@
 #!/bin/bash
-# round 6, visit 5: A/B of the three host-transfer modes against the read-only-page fault, the stress run on the staged library, the whole GPU suite, the top segment's weight in the
+# round 6, visit 5: the whole GPU suite, the top segment's weight in the
 # grouped form, two RCCL ranks on one device, a default bench run and its rocprofv3 kernel statistics
 O=gpurun_out/r6
 mkdir -p $O
-timeout 1500 python scripts/r6/fault_ab.py 12 > $O/v5_fault_ab.jsonl 2> $O/v5_fault_ab.err
-cat $O/v5_fault_ab.jsonl | cut -c1-400
-timeout 900 python scripts/r6/fault_stress.py 3 > $O/v5_stress.json 2> $O/v5_stress.err
-echo "stress rc=$?"; cat $O/v5_stress.json; grep -v host_pin $O/v5_stress.err | tail -n 3
 ( time timeout 1100 python -m pytest tests -x -q -m gpu -p no:cacheprovider ) > $O/v5_gpu_suite.log 2>&1
 tail -n 6 $O/v5_gpu_suite.log
 : > $O/v5_wtop_grouped.jsonl
