@@ -588,7 +588,8 @@ inline int user_compile(int32_t model, const std::vector<std::string>& exprs, st
         A.enter();
         if (A.CreateProgram(&prog, tu.c_str(), "hipadj_user_model.hip", NH, hptr, hnames) != HIPRTC_SUCCESS) { err = "hiprtcCreateProgram failed"; return HIPADJ_ERR_HIP; }
         for (const auto& e : exprs) A.AddNameExpression(prog, e.c_str());
-        std::vector<std::string> optv = {"--offload-arch=gfx950", (attempt == 0 && !low_opt) ? "-O3" : "-O1", "-std=c++17"};
+        std::vector<std::string> optv = {"--offload-arch=gfx950", (attempt == 0 && !low_opt) ? "-O3" : "-O1", "-std=c++17",
+                                         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"};      // as the library itself (build.py): some packed 32-bit forms have given wrong results here
         {   // adaptive Tsit5 of runtime models: the stage rows stay lane-private LDS columns.  The register form (hipadj_adaptive.hpp: KRegs) is 20-35 % faster here too
             // (runtime LV, 10^4 trajectories: Interpolating 0.51 -> 0.40 ms, Backsolve 0.47 -> 0.31; profiles/r3_tsit5_user_regs_ab.log), and every code object passed the
             // ISA check — but ONE of the suite's kernels came back with wrong parameter gradients (3-state ring, Interpolating, model cost, no tstops: GPU visit 22), the
