@@ -80,7 +80,7 @@ static void run(int pair, const Args& a, bool adjoint, bool wide, int form, bool
 }
 
 // the split of a problem: it depends on the sizes alone
-static int64_t tiles_of(const hipadj_recurrence* r, bool adjoint) { const int64_t rows = adjoint ? TTA : TTF; return std::max<int64_t>(1, (r->length + rows - 1) / rows); }
+static int64_t tiles_of(const hipadj_recurrence* r, bool adjoint) { const int64_t rows = adjoint ? TTA : TTF; return std::max<int64_t>(1, r->length / rows + (r->length % rows != 0)); }
 // Tiles of a group.  The exchange from group to group is what a few long chains wait for, and reading the group's earlier maps is what many chains pay for.  Measured with groups of 8, 16
 // and 32, forward and adjoint, BF16: 1 x 65536 x 128 (one chain) 53 / 36 / 31 and 95 / 62 / 48 us; 1 x 65536 x 512 (4 chains) 71 / 67 / 70 and 134 / 114 / 118; 1 x 65536 x 2048 (16 chains)
 // 206 / 207 / 213 and 357 / 363 / 372; 8 x 4096 x 2048 (128 chains) 97 / 98 / 96 and 162 / 168 / 176.
@@ -102,7 +102,7 @@ static int check(const hipadj_recurrence* r) {
     if (r->nseq > 0 && (r->batch != 1 || !r->offsets)) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: packed sequences (nseq > 0) need batch = 1 and offsets[nseq + 1]");
     if (r->nseq > 0 && r->offsets_bits != 32 && r->offsets_bits != 64) return ops_fail(HIPADJ_ERR_INVALID_ARG, "recurrence: offsets_bits must be 32 or 64");
     const int64_t ntiles = tiles_of(r, true);
-    const int64_t chains = r->channels ? (r->channels + 63) / 64 : 0;
+    const int64_t chains = r->channels / 64 + (r->channels % 64 != 0);
     if (r->batch && chains && ntiles > ((int64_t(1) << 31) - 1) / chains / r->batch) return ops_fail(HIPADJ_ERR_UNSUPPORTED, "recurrence: more than 2^31 - 1 tiles");
     return HIPADJ_OK;
 }
