@@ -268,7 +268,7 @@ class WideDeviceFunction(DeviceFunction):
             raise ValueError(f"dp must have shape ({self.np},), got {tuple(g.shape)}")
         if momentum is not None and (tuple(momentum.shape) != (self.np,) or momentum.dtype != torch.float32 or momentum.device != g.device or not momentum.is_contiguous()):
             raise ValueError(f"momentum must be a contiguous float32 tensor ({self.np},) on {g.device}")
-        g32, out = g.float(), torch.empty(self.np, dtype=torch.float32, device=g.device)
+        g32, out = g.float().contiguous(), torch.empty(self.np, dtype=torch.float32, device=g.device)
         for off, rows, cols in blocks:                       # column-major [rows x cols] is row-major [cols x rows], and the iteration commutes with transposition
             at, b = slice(off, off + rows * cols), slice(off + rows * cols, off + rows * cols + rows)
             view = lambda t: t[at].view(cols, rows)          # noqa: B023, E731
