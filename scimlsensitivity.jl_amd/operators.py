@@ -271,7 +271,10 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     for name, t, dt in (("momentum", momentum, torch.float32), ("out", out, grad.dtype)):
         if t is not None:
             _on(name, t, grad, dt, grad.shape)
-    co = [float(c) for row in coefficients for c in row] if len(coefficients) and not isinstance(coefficients[0], (int, float)) else [float(c) for c in coefficients] * int(steps)
+    try:
+        co = [float(c) for c in coefficients] * int(steps)
+    except TypeError:                                        # rows of three
+        co = [float(c) for row in coefficients for c in row]
     if len(co) != 3 * int(steps):
         raise ValueError(f"coefficients: three numbers, or three for each of the {steps} steps")
 

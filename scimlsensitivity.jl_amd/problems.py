@@ -273,7 +273,7 @@ class WideDeviceFunction(DeviceFunction):
             at, b = slice(off, off + rows * cols), slice(off + rows * cols, off + rows * cols + rows)
             view = lambda t: t[at].view(cols, rows)          # noqa: B023, E731
             operators.orthogonalized_update(view(g32), None if momentum is None else view(momentum), beta=beta, nesterov=nesterov, steps=steps,
-                                            coefficients=coefficients or operators.NEWTON_SCHULZ, scale=max(1.0, rows / cols) ** 0.5, out=view(out))
+                                            coefficients=operators.NEWTON_SCHULZ if coefficients is None else coefficients, scale=max(1.0, rows / cols) ** 0.5, out=view(out))
             if momentum is None:
                 out[b] = g32[b]
             else:
