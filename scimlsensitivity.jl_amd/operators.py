@@ -49,7 +49,8 @@ def _adjacent(t):
 
 
 def _rows(t):
-    """t with channels next to each other: as it is, or a copy."""
+    """t with channels next to each other: as it is, or a copy; a view whose sign torch has yet to turn (the imaginary part of a conjugate) with its sign turned."""
+    t = t.resolve_neg()
     return t if _adjacent(t) else t.contiguous()
 
 
@@ -71,6 +72,8 @@ def _written(torch, name, t):
     saved t says so."""
     if t.requires_grad and torch.is_grad_enabled():
         raise ValueError(f"{name} requires grad and is written in place, which has no gradient: call under torch.no_grad(), or pass {name}.detach()")
+    if t.is_neg():
+        raise ValueError(f"{name} is a view whose sign is yet to be turned (the imaginary part of a conjugate) and cannot be written in place: pass {name}.resolve_neg()")
     torch.autograd.graph.increment_version(t)
 
 
@@ -111,7 +114,7 @@ def recurrence_solve(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
         nseq = offsets.numel() - 1
     rows = nseq or batch
     if h0 is not None:
-        h0 = _on("h0", h0, x, wide, (rows, channels)).contiguous()
+        h0 = _on("h0", h0, x, wide, (rows, channels)).resolve_neg().contiguous()
     r = HipadjRecurrence()
     r.struct_size, r.device, r.dtype, r.gate_dtype = C.sizeof(HipadjRecurrence), x.device.index, _DTYPES[x.dtype], _DTYPES[gate.dtype]
     r.gate, r.coupled, r.batch, r.length, r.channels, r.nseq = GATES[form], int(bool(coupled)), batch, length, channels, nseq
@@ -151,7 +154,7 @@ def recurrence_adjoint(sol, dh=None, dh_final=None, *, need=(True, True, True)):
         dh = _rows(_on("dh", dh, x, x.dtype, x.shape))
         r.dh_stride[:] = _strides(dh, packed)
     if dh_final is not None:
-        dh_final = _on("dh_final", dh_final, x, sol._state_type, sol._final_shape).contiguous()
+        dh_final = _on("dh_final", dh_final, x, sol._state_type, sol._final_shape).resolve_neg().contiguous()
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
     dgate = torch.empty(gate.shape, dtype=gate.dtype, device=x.device) if need[1] else None
     dh0 = torch.empty(sol._final_shape, dtype=sol._state_type, device=x.device) if need[2] else None
@@ -201,7 +204,7 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
                 for name, t, (dtype, shape, device) in zip(("x", "gate", "h0", "offsets", "the checkpoints"), ctx.saved_tensors, ctx.kinds):
                     if t is not None and (t.dtype, t.shape, t.device) != (dtype, shape, device):
                         raise ValueError(f"{name} was saved as {dtype} {tuple(shape)} on {device} and came back as {t.dtype} {tuple(t.shape)} on {t.device}")
-                    saved.append(t if t is None else _rows(t) if name in ("x", "gate") else t.contiguous())
+                    saved.append(t if t is None else _rows(t) if name in ("x", "gate") else t.resolve_neg().contiguous())
                 sol.x, sol.gate, sol.h0, sol.offsets, sol._checkpoints = saved
                 sol.form, sol.coupled, sol._config, sol._workspace_bytes, sol._state_type, sol._final_shape, sol._stream = ctx.rest
                 dx, dgate, dh0 = recurrence_adjoint(sol, dh, dh_final, need=ctx.needs_input_grad[:3])
@@ -286,7 +289,7 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
         except RuntimeError:
             return None
 
-    given_out = out
+    given_out, grad = out, grad.resolve_neg()
     if out is None:
         out = torch.empty(grad.shape, dtype=grad.dtype, device=grad.device) if grad.stride(-1) == 1 or grad.stride(-2) != 1 else \
             torch.empty((*grad.shape[:-2], grad.shape[-1], grad.shape[-2]), dtype=grad.dtype, device=grad.device).transpose(-1, -2)

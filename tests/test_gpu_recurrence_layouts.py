@@ -34,3 +34,24 @@ def test_results_keep_the_order_of_batch_and_time(sa, torch):
     x = torch.randn(40, 3, 16, device="cuda").transpose(0, 1)
     sol = sa.recurrence_solve(x, -x.abs(), form="log")
     assert sol.h.stride() == x.stride() and torch.equal(sol.h, sa.recurrence_solve(x.contiguous(), -x.abs().contiguous(), form="log").h)
+
+
+def test_views_whose_sign_is_yet_to_be_turned(sa, torch):
+    """The imaginary part of a conjugate is a view of the other sign: one channel, where its stride does not ask for a copy, and several."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    for channels in (1, 4):
+        parts = [torch.complex(*torch.randn(2, 1, 30, channels, device="cuda", generator=gen)).conj().imag for _ in range(3)]
+        starts = [torch.complex(*torch.randn(2, 1, channels, device="cuda", generator=gen)).conj().imag for _ in range(2)]
+        assert all(t.is_neg() for t in parts + starts)
+        results = []
+        for turn in (lambda t: t, lambda t: t.resolve_neg().clone()):
+            x, g, dh, h0, last = (turn(t) for t in parts + starts)
+            sol = sa.recurrence_solve(x, g, h0, form="sigmoid", coupled=True)
+            results.append([sol.h, sol.h_final, *sa.recurrence_adjoint(sol, dh, last), sa.gated_recurrence_step(x[0], g[0], torch.ones(30, channels, device="cuda"), form="sigmoid"),
+                            sa.orthogonalized_update(x), sa.orthogonalized_update(x.transpose(1, 2))])
+        assert all(torch.equal(a, b) for a, b in zip(*results))
+        # (with several channels these views have strides of two, for which they are refused before their sign)
+        with pytest.raises(ValueError, match="sign is yet" if channels == 1 else "neighbouring channels"):
+            sa.gated_recurrence_step(parts[0][0], parts[1][0], parts[2][0])
+        with pytest.raises(ValueError, match="sign is yet" if channels == 1 else "row-major"):
+            sa.orthogonalized_update(parts[0].resolve_neg(), out=parts[1])
