@@ -244,7 +244,9 @@ def _disjoint(t):
     """Whether no two elements of t [batch, rows, cols] share a place, for a t with columns or rows next to each other (others are refused for that)."""
     if t.numel() == 0:
         return True
-    t = t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.transpose(-1, -2)
+    t = t if _adjacent(t) else t.transpose(-1, -2)
+    if not _adjacent(t):
+        return True
     (batch, rows, cols), (sb, sr, _) = t.shape, t.stride()
     if rows > 1 and sr < cols:
         return False

@@ -31,5 +31,7 @@ def test_overlapping_rows_are_refused(sa):
         for kw in (dict(momentum=bad), dict(out=bad)):
             with pytest.raises(ValueError, match="not overlap"):
                 sa.orthogonalized_update(g, **kw)
+    with pytest.raises(ValueError, match="both be row-major"):                 # neither columns nor rows next to each other: refused for that
+        sa.orthogonalized_update(g, out=z(2, 5, 8)[..., ::2])
     heads = z(5, 2, 4).transpose(0, 1)                                         # matrices side by side
     assert sa.orthogonalized_update(g, out=heads) is heads and sa.orthogonalized_update(z(2, 4, 5).transpose(1, 2), z(2, 4, 5).transpose(1, 2)).shape == g.shape
