@@ -460,7 +460,9 @@ typedef enum { HIPADJ_GATE_DECAY = 0, HIPADJ_GATE_LOG = 1, HIPADJ_GATE_SIGMOID =
  *   packed  nseq > 0, batch = 1: sequence s is the rows offsets[s] <= t < offsets[s + 1] (device memory, ascending; equal neighbours: an empty sequence, whose final state is its
  *           first); h0, h_final, dh_final, dh0 [nseq][channels].  Rows of no sequence have h = 0 and zero gradients and are not used.  Offsets that do not ascend or pass `length` give
  *           unspecified results, never an access outside the arrays.
- *           Decays above one are taken as they are; where their product over some hundred rows overflows, so may a state that row by row would not yet.
+ *           Decays above one are taken as they are; where their product over some hundred rows overflows, so may a state that row by row would not yet, and a decay of zero behind
+ *           it makes it NaN.  A state that is infinite stays so, but turns NaN where the product of 16 rows' decays (adjoint: 8) is below the smallest number there is.
+ *           No output may overlap an input or another output.
  * dtype: x, h, dh, dx; gate_dtype: gate, dgate — the same, or F32 next to BF16 / F16.  h0, h_final, dh_final, dh0 and the checkpoints: F64 for F64, else F32, contiguous.  States and
  * gradients are carried in that type, the outputs rounded once.
  *   hipadj_recurrence_sizes         bytes of the checkpoints and of the workspace (8-byte aligned; 0: none) of a configuration
@@ -469,7 +471,8 @@ typedef enum { HIPADJ_GATE_DECAY = 0, HIPADJ_GATE_LOG = 1, HIPADJ_GATE_SIGMOID =
  *                                   checkpoint interval is re-solved
  *   hipadj_recurrence_step_dev      one step of `batch` sequences: state[slots[i]] <- a state[slots[i]] + b, h[i] = the new state; x, gate, h [batch][channels], state [nslots][channels]
  *                                   (F64 for F64, else F32) with row strides; slots NULL: row i has state i.  A slot outside [0, nslots) is padding: h[i] = 0.  Rows with the same
- *                                   slot are consecutive steps of it in row order.  h may not overlap another argument. */
+ *                                   slot are consecutive steps of it in row order (each row looks at all slots: batch^2 reads for a row of channels).  h may not overlap another
+ *                                   argument, nor state x or gate. */
 typedef struct {
     uint32_t struct_size;      /* = sizeof(hipadj_recurrence) */
     int32_t device;

@@ -216,7 +216,8 @@ def gated_recurrence(x, gate, h0=None, *, form="log", coupled=False, offsets=Non
 def gated_recurrence_step(x, gate, state, *, form="log", coupled=False, slots=None):
     """One step of running sequences: state[slots[i]] <- a state[slots[i]] + b in place, and h[i] = the new state in x's type.  x, gate [batch][channels]; state
     [nslots][channels] float32 (float64 for float64); slots int32 / int64 [batch] or None (row i has state i).  A slot outside the states (-1) pads the batch: h[i] = 0.
-    Rows with the same slot are consecutive steps of that state in row order.  No gradients: gated_recurrence over one row has them; a state that requires grad is refused in grad mode."""
+    Rows with the same slot are consecutive steps of that state in row order.  No gradients: gated_recurrence over one row has them; a state that requires grad is refused in grad mode.  x and gate may not
+    lie in state."""
     torch = _torch()
     if x.dim() != 2:
         raise ValueError(f"x must be [batch][channels], got shape {tuple(x.shape)}")
