@@ -507,7 +507,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 
 // ---- adjoint ------------------------------------------------------------------------------------------------------------------------------------------------------
 // Where both a and 1 - a are needed, 16-bit data keep the smaller one in registers, with its own digits, and the larger one is its difference from one, good to half a unit: both are factors
-// of gradients, and 1 - (1 - a) would have none of a's digits left at exp(-17).  Wider data keep a and evaluate the gate again at the end.  16-bit data also leave x and dh
+// of gradients, and 1 - (1 - a) would have none of a's digits left at exp(-17).  (Packed rows keep both: their scalar registers have no room for the masks, which made 87 us of 65-68.)  Wider
+// data keep a and evaluate the gate again at the end.  16-bit data also leave x and dh
 // as they arrived and make 32-bit values of them each time they are used (`again` hides that they are the same values), and read dh a second time, from L2: then three workgroups share
 // a CU instead of two (80 registers), and the adjoint of 8 x 4096 x 2048 BF16 takes 164 us instead of 180.  (Not for packed rows where 1 - a is kept: 13-29 registers would spill, 64-75 us
 // for 37 ... 512 sequences of 16384 x 1024 F16 against 64-80.)
@@ -538,11 +539,15 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
     if constexpr (PACKED) m = marks_of<TS>(p, t0, win, seqs[wave]);
     const uint32_t cuts = PACKED ? (m.start | m.out) : 0;
     arrived(rg); arrived(rx); arrived(rd);
-    S kept[TS][V], before[TS][V];                             // a or (PAIR) the smaller of a and 1 - a of each row; the state before it, till then its b unless that is made again from x (LATE)
-    constexpr bool PAIR = KEEP && FORM != 0;                  // (a given decay is kept itself, 1 - a is its difference from one by definition)
+    constexpr bool PAIR = KEEP && FORM != 0, BOTH = PAIR && PACKED;      // (a given decay is kept itself, 1 - a is its difference from one by definition)
+    S kept[TS][V], rests[BOTH ? TS : 1][V];                   // a or (PAIR) the smaller of a and 1 - a of each row, or both
+    S before[TS][V];                                          // the state before each row; till then its b unless that is made again from x (LATE)
     bool low[TS][V];                                          // PAIR: a is what is kept: a mask a row in scalar registers
     auto a = [&](int i, int v) -> S { return PAIR && !low[i][v] ? S(1) - kept[i][v] : kept[i][v]; };
-    auto rest_of = [&](int i, int v) -> S { return PAIR && !low[i][v] ? kept[i][v] : S(1) - kept[i][v]; };      // KEEP
+    auto rest_of = [&](int i, int v) -> S {                   // KEEP
+        if constexpr (BOTH) return rests[i][v];
+        else return PAIR && !low[i][v] ? kept[i][v] : S(1) - kept[i][v];
+    };
     auto b_of = [&](int i, int v) -> S {
         if constexpr (!LATE) return before[i][v];
         const S x = (S)part<T, V>(rx[i], v);
@@ -552,7 +557,7 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         if constexpr (sizeof(T) == 2) arrived(rx);
         if constexpr (KEEP)
 #pragma unroll
-            for (int i = 0; i < TS; ++i) arrived(kept[i]);
+            for (int i = 0; i < TS; ++i) { arrived(kept[i]); if constexpr (BOTH) arrived(rests[i]); }
     };
     auto at_seq = [&](const void* of, int i, int v) -> S {    // of the sequence that row i belongs to, in h0 or dh_final
         const int64_t s = uniform(seqs[wave][i]);
@@ -573,8 +578,9 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         for (int v = 0; v < V; ++v) {
             S aa, rest = S(0);
             decay<FORM, REST, FAST, S>((S)part<TG, V>(rg[i], v), aa, rest);
-            low[i][v] = PAIR && aa < S(0.5);
+            low[i][v] = PAIR && (BOTH || aa < S(0.5));
             kept[i][v] = PAIR && !low[i][v] ? rest : aa;
+            if constexpr (BOTH) rests[i][v] = rest;
             if constexpr (!LATE) before[i][v] = rest * (S)part<T, V>(rx[i], v);
         }
     if (rows < TS) {                                          // rows behind the end pass a state on
@@ -582,7 +588,7 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
         for (int i = 0; i < TS; ++i) if (i >= rows) {
             rx[i] = 0; rd[i] = 0;
 #pragma unroll
-            for (int v = 0; v < V; ++v) { low[i][v] = false; kept[i][v] = PAIR ? S(0) : S(1); if constexpr (!LATE) before[i][v] = S(0); }
+            for (int v = 0; v < V; ++v) { low[i][v] = BOTH; kept[i][v] = PAIR && !BOTH ? S(0) : S(1); if constexpr (BOTH) rests[i][v] = S(0); if constexpr (!LATE) before[i][v] = S(0); }
         }
     }
     if constexpr (PACKED) if (m.out) {
