@@ -265,7 +265,8 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     (nesterov) or momentum, X = u / (|u| + 1e-7), `steps` times X <- c0 X + c1 A X + c2 A A X with A = X X', and scale X is returned in grad's type.
 
     grad [..., rows, cols] float32, bfloat16 or float16: every matrix of the leading dimensions by itself (heads, layers); row-major or its transpose.
-    coefficients: three numbers, or three for each step.  out: where to write (like grad; grad itself is allowed); neither momentum nor out may require grad in grad mode.  For weights W [out, in] the usual step is
+    coefficients: three numbers, or three for each step.  out: where to write (like grad; grad itself is allowed); momentum may overlap
+    neither, and neither momentum nor out may require grad in grad mode.  For weights W [out, in] the usual step is
     W -= lr * orthogonalized_update(dW, m, scale=max(1, out / in) ** 0.5)."""
     torch = _torch()
     if not grad.is_cuda:
@@ -322,6 +323,8 @@ def orthogonalized_update(grad, momentum=None, *, beta=0.95, nesterov=True, step
     L = _lib.load()
     ws = C.c_int64()
     _check(L.hipadj_orthogonalized_update_size(C.byref(q), C.byref(ws)))
+    if m is not None and m.numel() and m.data_ptr() in (g.data_ptr(), o.data_ptr()):
+        raise ValueError("momentum is written in place and may not be grad or out")
     for name, t in (("momentum", momentum), ("out", given_out)):
         if t is not None:
             _written(torch, name, t)

@@ -35,3 +35,17 @@ def test_overlapping_rows_are_refused(sa):
         sa.orthogonalized_update(g, out=z(2, 5, 8)[..., ::2])
     heads = z(5, 2, 4).transpose(0, 1)                                         # matrices side by side
     assert sa.orthogonalized_update(g, out=heads) is heads and sa.orthogonalized_update(z(2, 4, 5).transpose(1, 2), z(2, 4, 5).transpose(1, 2)).shape == g.shape
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 5, 4), (200, 150)])
+def test_momentum_in_the_place_of_another_argument_is_refused(sa, shape):
+    g = torch.randn(*shape, device="cuda")
+    m = torch.randn(*shape, device="cuda")
+    before = g.clone(), m.clone()
+    for call in (lambda: sa.orthogonalized_update(g, g), lambda: sa.orthogonalized_update(g, m, out=m), lambda: sa.orthogonalized_update(g.transpose(-1, -2), g.transpose(-1, -2))):
+        with pytest.raises(ValueError, match="momentum is written in place"):
+            call()
+    assert torch.equal(g, before[0]) and torch.equal(m, before[1])
+    want = sa.orthogonalized_update(g.clone(), m.clone())
+    assert torch.equal(sa.orthogonalized_update(g, m, out=g), want) and torch.equal(g, want)
