@@ -45,3 +45,26 @@ def test_a_solution_dropped_while_its_adjoint_waits_on_another_stream(sa, torch,
         side.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         del over
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_an_adjoint_captured_of_an_eager_solution(sa, torch, packed):
+    """The solution belongs to the default stream, its adjoint to a captured graph: every replay gives the eager gradients, also after new cotangents, with eager work between."""
+    gen = torch.Generator("cuda").manual_seed(6)
+    x, gate, dh = (torch.randn(2, 300, 40, device="cuda", generator=gen) for _ in range(3))
+    kw = {}
+    if packed:
+        x, gate, dh, kw = x[0], gate[0], dh[0], dict(offsets=torch.tensor([0, 100, 290], device="cuda"))
+    sol = sa.recurrence_solve(x, gate, form="sigmoid", **kw)
+    sa.recurrence_adjoint(sol, dh)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sa.recurrence_adjoint(sol, dh)
+    for i in range(4):
+        dh.copy_(torch.randn(dh.shape, device="cuda", generator=gen))
+        graph.replay()
+        want = sa.recurrence_adjoint(sol, dh)
+        busy(torch, 2)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
