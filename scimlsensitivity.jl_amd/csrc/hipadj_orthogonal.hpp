@@ -154,8 +154,9 @@ template <class T, bool SPLIT, int WAVES> __global__ void __launch_bounds__(WAVE
 // In a stage the factors of its second half are read while the first half is multiplied, and those of the next stage's first half while the second is; the one barrier stands between the
 // halves: behind it the next stage has arrived in every wave's part, and no wave still reads this stage's buffer, which stage s + 4 is requested into.
 //
-// Bound: the matrix cores, at the clock that the board's power leaves (1.95 GHz while they are busy).  4096 x 4096, one term: X X' and the polynomial of A, half their tiles each, 92 and 96 us
-// (750 and 715 TFLOP/s of the half), B X with X out in three forms 147-163 us (840-930).  Small sides: a launch of 4-9 us each, most of it the latency of the first stages and of the
+// Measured, 4096 x 4096, one term: X X' and the polynomial of A, half their tiles each, 92 and 96 us (745 and 715 TFLOP/s of the half), B X with X out in three forms 156-164 us (840-880).  The
+// matrix cores are busy 41-49 % of that time (31 % of B X and 21 % of X X' at 2048 x 8192); a library product of 4096 keeps them busy 72 % of 99 us at the same 1.8-1.9 GHz, so it is not the
+// clock: one workgroup a CU leaves them idle during its first stages and its epilogue, and B X stores 8 bytes an element there.  Small sides: a launch of 4-9 us each, most of it the latency of the first stages and of the
 // epilogue (two groups of four waves that share a tile and halve K were 10 % slower at every size).
 enum { GRAM = 0, POLY = 1, APPLY = 2, LAST = 3, PARTS = 4, JOIN = 5 };        // PARTS, JOIN: GRAM in two launches, parts of K and their sum (in the order of the parts)
 

@@ -21,10 +21,11 @@
 // registers — the bytes of reading h back are those of reading x, and the states are the unrounded ones.
 // Bound: memory, 3 streams forward and 5 in the adjoint, where the axes are long and many; the exchanges along the chain where there are few.  Measured on an MI355X (a copy: 5.10 TB/s), the
 // launch of k_zero (2-6 us) not counted:
-//   forward  1 x 65536 x 2048 BF16, exp gate            194 us, 4.16 TB/s        8 x 4096 x 2048 BF16, coupled sigmoid, with checkpoints   98 us, 4.15 TB/s
-//            37 packed sequences, 16381 x 1024 F16       36 us, 2.8 TB/s         2 x 2047 x 777 F32                                        16 us, 2.5 TB/s
-//            1 x 512 x 2048 BF16                        8.8 us: four tiles a chain, latency
-//   adjoint  8 x 4096 x 2048 BF16, coupled sigmoid      164 us, 4.1 TB/s         2 x 2047 x 777 F32                                        26 us, 2.4 TB/s
+//   forward  1 x 65536 x 2048 BF16, exp gate            197 us, 4.09 TB/s        8 x 4096 x 2048 BF16, coupled sigmoid, with checkpoints  103 us, 3.95 TB/s
+//            37 packed sequences, 16381 x 1024 F16       40 us, 2.5 TB/s         2 x 2047 x 777 F32                                        16 us, 2.4 TB/s
+//            1 x 512 x 2048 BF16                        9.1 us: four tiles a chain, latency
+//   adjoint  8 x 4096 x 2048 BF16, coupled sigmoid      185 us, 3.7 TB/s         2 x 2047 x 777 F32                                        27 us, 2.3 TB/s
+// (averages of 13 calls; the vector units are busy 41 % of the time in the first of these, 55 % in the second and 74 % in the adjoint of 16-bit data).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -510,8 +511,8 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : 4) k_forward(const Ar
 // of gradients, and 1 - (1 - a) would have none of a's digits left at exp(-17).  (Packed rows keep both: their scalar registers have no room for the masks, which made 87 us of 65-68.)  Wider
 // data keep a and evaluate the gate again at the end.  16-bit data also leave x and dh
 // as they arrived and make 32-bit values of them each time they are used (`again` hides that they are the same values), and read dh a second time, from L2: then three workgroups share
-// a CU instead of two (80 registers), and the adjoint of 8 x 4096 x 2048 BF16 takes 164 us instead of 180.  (Not for packed rows where 1 - a is kept: 13-29 registers would spill, 64-75 us
-// for 37 ... 512 sequences of 16384 x 1024 F16 against 64-80.)
+// a CU instead of two (80 registers), and the adjoint of 8 x 4096 x 2048 BF16 takes 185 us instead of 204 (two workgroups a CU with both values in registers).  Packed rows that keep both
+// have two: 69-83 us for 37 ... 512 sequences of 16384 x 1024 F16.
 template <class T, class TG, class S, int V, int FORM, bool COUPLED, bool PACKED>
 __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && sizeof(TG) == 2 && !(PACKED && (COUPLED || FORM == 2)) ? 6 : 4) k_adjoint(const Args p) {
     __shared__ Lds<S, V> sh;
@@ -726,7 +727,7 @@ __global__ void __launch_bounds__(NT, sizeof(S) == 8 ? 2 : sizeof(T) == 2 && siz
 // ---- single step --------------------------------------------------------------------------------------------------------------------------------------------------
 // One row per sequence: state[slot] = a state[slot] + b, h = the new state.  Rows that name the same slot are steps of one sequence in the order of the rows: the first of them
 // takes all, so no two workgroups touch a state.  A slot outside [0, nslots) (-1 pads a batch) has no state: its h is zero.
-// A row is read, updated and written by neighbouring lanes of workgroups of their own: 14 bytes a BF16 channel.  256 rows x 4096 channels 6.6 us (2.2 TB/s; a launch alone is 2.2 us, which
+// A row is read, updated and written by neighbouring lanes of workgroups of their own: 14 bytes a BF16 channel.  256 rows x 4096 channels 6.7 us (2.2 TB/s; a launch alone is 2.2 us, which
 // is one row of 2048 channels).
 struct StepArgs {
     const void *x, *gate, *slots;

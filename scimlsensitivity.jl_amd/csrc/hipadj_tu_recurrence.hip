@@ -83,7 +83,8 @@ static void run(int pair, const Args& a, bool adjoint, bool wide, int form, bool
 static int64_t tiles_of(const hipadj_recurrence* r, bool adjoint) { const int64_t rows = adjoint ? TTA : TTF; return std::max<int64_t>(1, r->length / rows + (r->length % rows != 0)); }
 // Tiles of a group.  The exchange from group to group is what a few long chains wait for, and reading the group's earlier maps is what many chains pay for.  Measured with groups of 8, 16
 // and 32, forward and adjoint, BF16: 1 x 65536 x 128 (one chain) 53 / 36 / 31 and 95 / 62 / 48 us; 1 x 65536 x 512 (4 chains) 71 / 67 / 70 and 134 / 114 / 118; 1 x 65536 x 2048 (16 chains)
-// 206 / 207 / 213 and 357 / 363 / 372; 8 x 4096 x 2048 (128 chains) 97 / 98 / 96 and 162 / 168 / 176.
+// 206 / 207 / 213 and 357 / 363 / 372; 8 x 4096 x 2048 (128 chains) 97 / 98 / 96 and 162 / 168 / 176.  (All before maps passed exactly and the adjoint kept small decays; the chosen ones are
+// 31, 50; 66, 115; 204, 358 and 107, 185 since.)
 static int group_of(int64_t nchains) { return nchains <= 2 ? 32 : nchains <= 4 ? 16 : 8; }
 // 64-bit words of a launch: the ticket, a map for each tile, a state for each group, by channel
 static int64_t words_of(const hipadj_recurrence* r, int64_t ntiles, int V) {
